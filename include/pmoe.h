@@ -328,6 +328,110 @@ PMOE_API int pmoe_expert_ffn_backward(const void* grad_out, const void* hidden, 
                                       void* grad_gate_up_proj, void* grad_down_proj, int grad_weight_dtype,
                                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------- router auxiliary loss ---
+ * The balance loss, the z-loss and the per-expert counts of all layers' router
+ * logits at once, with every layer's gradient: Qwen3Moe.aux_loss and
+ * _update_expert_counts (qwen3_moe.py:417-444) over load_balancing_loss and
+ * router_z_loss (:285-316). With p = softmax(l_t) in fp32, S_t the top_k
+ * largest logits of row t (equal logits: the lower expert id; NaN above all, as
+ * torch sorts), c_e = the number of valid rows of all layers with e in S_t and n
+ * the number of valid rows:
+ *   LB = E sum_e (c_e / n) (sum_t p_te / n),   Z = sum_t lse_t^2 / n,
+ *   loss = aux_coef LB + z_coef Z, load_balance = LB, z_loss = Z
+ * (one fp32 each in device memory). No valid row: all three are 0. logits: a HOST array of L device pointers, each
+ * (rows[i], E) of `dtype` (fp32, bf16 or fp16), row_counts a HOST array of L.
+ * mask: (mask_rows,) bytes or NULL; a row whose byte is 0 counts for nothing,
+ * whatever it holds, in every layer (each then has mask_rows rows).
+ * expert_counts: (L, E) int32; coef: (E + 1,) fp32 that the backward takes. The
+ * sums have a fixed order: the same inputs give the same bits. */
+PMOE_API size_t pmoe_aux_loss_forward_workspace_size(const int64_t* row_counts, int64_t L, int64_t E);
+PMOE_API int pmoe_aux_loss_forward(const void* const* logits, const int64_t* row_counts, int64_t L, int dtype,
+                                   const uint8_t* mask, int64_t mask_rows, int64_t E, int64_t K, float aux_coef,
+                                   float z_coef, float* loss, float* load_balance, float* z_loss, int32_t* expert_counts, float* coef, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* The same values from the statistics that pmoe_router_forward emits (no pass
+ * over the logits): HOST arrays of L device pointers to each layer's
+ * expert_counts (E,) int32, prob_sum (E,) fp32 and lse_sq_sum (1,) fp32, and n,
+ * the rows of all layers. K is the routers' top_k. */
+PMOE_API size_t pmoe_aux_loss_from_stats_workspace_size(int64_t L, int64_t E);
+PMOE_API int pmoe_aux_loss_from_stats(const int32_t* const* layer_counts, const float* const* prob_sums,
+                                      const float* const* lse_sq_sums, int64_t L, int64_t n, int64_t E, int64_t K,
+                                      float aux_coef, float z_coef, float* loss, float* load_balance, float* z_loss, int32_t* expert_counts, float* coef,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradient of loss times grad_loss (1,) fp32 in device memory: into
+ * grads[i] (HOST array of L device pointers; NULL: not wanted), shaped and typed
+ * as logits[i]:
+ *   dl_tj = grad_loss p_tj [aux_coef E / n (f_j - sum_e f_e p_te) + 2 z_coef / n lse_t],
+ * f_e = c_e / n (the counts carry no gradient, as the reference's one-hot
+ * selection does not); rows masked out get zeros. coef is the forward's. */
+PMOE_API int pmoe_aux_loss_backward(const void* const* logits, void* const* grads, const int64_t* row_counts,
+                                    int64_t L, int dtype, const uint8_t* mask, int64_t mask_rows, int64_t E,
+                                    const float* coef, const float* grad_loss, float aux_coef, float z_coef,
+                                    void* stream);
+
+/* ------------------------------------------------------------ layer norm ---
+ * torch.nn.LayerNorm over the last dimension, beside the RMSNorm that the
+ * reference's blocks use (qwen3_moe.py:260): mu = mean(x[t]), r = 1 /
+ * sqrt(mean((x[t] - mu)^2) + eps), out[t] = (x[t] - mu) r weight + bias, fp32
+ * arithmetic. x (T,H) x_dtype; weight and bias (H,) w_dtype or NULL (1 and 0);
+ * out (T,H) out_dtype: x_dtype, or 16 bits from fp32 x; mean and rstd (T,) fp32,
+ * or both NULL. Any H >= 1 (rows of 16-byte pieces are read as such, others
+ * element by element); T < 2^24. */
+PMOE_API int pmoe_layernorm_forward(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype,
+                                    float eps, int64_t T, int64_t H, void* out, int out_dtype, float* mean,
+                                    float* rstd, void* stream);
+
+/* Its backward, xh = (x - mean) rstd:
+ *   grad_x = rstd (g w - mean(g w) - xh mean(g w xh)),
+ *   grad_weight = sum_t g xh, grad_bias = sum_t g (fixed-order partial sums).
+ * grad (T,H) grad_dtype, the forward's out_dtype; grad_x (T,H) x_dtype;
+ * grad_weight and grad_bias (H,) w_dtype. Each of the three may be NULL. With T =
+ * 0 the weight's and the bias's gradients are zeros. */
+PMOE_API size_t pmoe_layernorm_backward_workspace_size(int64_t T, int64_t H);
+PMOE_API int pmoe_layernorm_backward(const void* grad, int grad_dtype, const void* x, int x_dtype, const void* weight,
+                                     int w_dtype, const float* mean, const float* rstd, int64_t T, int64_t H,
+                                     void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/* ------------------------------------- activation checkpoints in 8 bits ---
+ * A tensor kept for the backward in 8 bits: the columns of a row in groups of 32
+ * (the last may be shorter), one power of two per group. With a the group's
+ * largest finite magnitude, e = the least integer >= -126 with rint(a 2^-e) <=
+ * 127, codes = rint(x 2^-e) (ties to even), exps = e + 127; a value that is not
+ * finite has code -128. Restored: code 2^e, at most the type's largest finite
+ * magnitude, and NaN for -128. The error is at most 2^(e-1) <= a / 127.
+ * x (R,C) of `dtype`; codes (R,C) int8; exps (R, ceil(C / 32)) bytes. */
+PMOE_API int pmoe_act8_save(const void* x, int dtype, int64_t R, int64_t C, int8_t* codes, uint8_t* exps,
+                            void* stream);
+PMOE_API int pmoe_act8_restore(const int8_t* codes, const uint8_t* exps, int64_t R, int64_t C, void* x, int dtype,
+                               void* stream);
+
+/* pmoe_gate_up_swiglu with gate_up_out kept in 8 bits: codes (P, 2I) int8 and
+ * exps (P, 2, ceil(I / 32)) bytes, of the values that gate_up_out would have had
+ * (the groups of gate and of up are apart). mid is pmoe_gate_up_swiglu's, bit for
+ * bit. The workspace holds gate_up_out where the product does not write the
+ * codes itself. */
+PMOE_API size_t pmoe_gate_up_swiglu_act8_workspace_size(int64_t P, int64_t E, int64_t H, int64_t I, int dtype);
+PMOE_API int pmoe_gate_up_swiglu_act8(const void* x, const int32_t* row_index, const float* row_weight, int64_t x_rows,
+                                      const void* gate_up_proj, const int32_t* offs, int dtype, int64_t P, int64_t E,
+                                      int64_t H, int64_t I, int8_t* codes, uint8_t* exps, void* mid, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* The input gradient of pmoe_down_proj through the SwiGLU (grad_gate_up_out and
+ * part of pmoe_down_proj_backward) with gate and up restored from their 8-bit
+ * checkpoint, and the activation computed again from them: mid (P, I) =
+ * row_weight * silu(gate) * up, for the weight gradient (or NULL). The workspace
+ * holds the restored gate_up_out (and mid, where mid is NULL) where the product
+ * does not read the codes itself. */
+PMOE_API size_t pmoe_down_proj_dgrad_act8_workspace_size(int64_t P, int64_t E, int64_t H, int64_t I, int dtype);
+PMOE_API int pmoe_down_proj_dgrad_act8(const void* grad, const int32_t* row_index, const float* row_weight,
+                                       int64_t grad_rows, const int8_t* codes, const uint8_t* exps,
+                                       const void* down_proj, const int32_t* offs, int dtype, int64_t P, int64_t E,
+                                       int64_t H, int64_t I, void* grad_gate_up_out, void* mid, float* part,
+                                       int64_t part_ld, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------- engine queries ---
  * No counterpart in the reference (which has no kernels of its own): which
  * tile the grouped-GEMM engine gives an expert GEMM, for tests and tuning.

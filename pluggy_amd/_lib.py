@@ -6,6 +6,7 @@ the library is missing, or a tensor is not on a ROCm device, calls raise.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -57,6 +58,23 @@ SIGNATURES = {
     "pmoe_dispatch_rmsnorm_backward_workspace_size": (_SZ, [_I64, _I64]),
     "pmoe_dispatch_rmsnorm_backward": (_INT, [_P, _P, _P, _INT, _P, _INT, _P, _P, _P, _I64, _I64, _I64, _P, _P,
                                               _INT, _P, _SZ, _P]),
+    "pmoe_aux_loss_forward_workspace_size": (_SZ, [_P, _I64, _I64]),
+    "pmoe_aux_loss_forward": (_INT, [_P, _P, _I64, _INT, _P, _I64, _I64, _I64, _F32, _F32, _P, _P, _P, _P, _P, _P, _SZ,
+                                     _P]),
+    "pmoe_aux_loss_from_stats_workspace_size": (_SZ, [_I64, _I64]),
+    "pmoe_aux_loss_from_stats": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _F32, _F32, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "pmoe_aux_loss_backward": (_INT, [_P, _P, _P, _I64, _INT, _P, _I64, _I64, _P, _P, _F32, _F32, _P]),
+    "pmoe_layernorm_forward": (_INT, [_P, _INT, _P, _P, _INT, _F32, _I64, _I64, _P, _INT, _P, _P, _P]),
+    "pmoe_layernorm_backward_workspace_size": (_SZ, [_I64, _I64]),
+    "pmoe_layernorm_backward": (_INT, [_P, _INT, _P, _INT, _P, _INT, _P, _P, _I64, _I64, _P, _P, _P, _P, _SZ, _P]),
+    "pmoe_act8_save": (_INT, [_P, _INT, _I64, _I64, _P, _P, _P]),
+    "pmoe_act8_restore": (_INT, [_P, _P, _I64, _I64, _P, _INT, _P]),
+    "pmoe_gate_up_swiglu_act8_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _INT]),
+    "pmoe_gate_up_swiglu_act8": (_INT, [_P, _P, _P, _I64, _P, _P, _INT, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ,
+                                        _P]),
+    "pmoe_down_proj_dgrad_act8_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _INT]),
+    "pmoe_down_proj_dgrad_act8": (_INT, [_P, _P, _P, _I64, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _P, _P, _P,
+                                         _I64, _P, _SZ, _P]),
     "pmoe_expert_ffn_forward_workspace_size": (_SZ, [_I64, _I64, _I64]),
     "pmoe_expert_ffn_forward": (_INT, [_P, _P, _P, _INT, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _P, _P,
                                        _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
@@ -127,6 +145,14 @@ def require_gpu(*tensors: torch.Tensor) -> None:
         if t is not None and not t.is_cuda:
             raise RuntimeError("pluggy_amd runs on ROCm GPU tensors only (there is no CPU fallback); "
                                f"got a tensor on {t.device}")
+
+
+def on_device(t: torch.Tensor):
+    """Context that makes ``t``'s device the current one (launches go to the
+    current device, a stream belongs to one)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def workspace(nbytes: int, device) -> torch.Tensor:

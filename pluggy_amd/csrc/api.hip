@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include "../../include/pmoe.h"
+#include "act8.h"
 #include "kernels.h"
 
 using namespace pmoe;
@@ -944,6 +945,336 @@ PMOE_API int pmoe_dispatch_rmsnorm_backward(const void* grad_x_perm, const int32
     PMOE_TRY(st, "dispatch_rmsnorm_backward (weight)");
   }
   return PMOE_OK;
+}
+
+// -------------------------------------------------- router auxiliary loss
+
+extern "C++" {
+namespace {
+
+struct AuxPlan {
+  int bpl = 1;       // blocks of a layer
+  int64_t rows = 0;  // most rows of a layer
+};
+
+int check_aux(const void* const* arrays, const int64_t* rows, int64_t L, int64_t E, int64_t K, const char* what,
+              AuxPlan* plan) {
+  PMOE_REQUIRE(L >= 1 && L <= 4096, "%s: %lld layers (1 to 4096 are supported)", what, (long long)L);
+  if (int rc = check_moe_dims(0, K, E, 8, 0)) return rc;
+  PMOE_REQUIRE(arrays && rows, "%s: null array", what);
+  int64_t total = 0;
+  for (int64_t i = 0; i < L; ++i) {
+    PMOE_REQUIRE(rows[i] >= 0 && rows[i] <= kMaxIndex, "%s: layer %lld has %lld rows", what, (long long)i,
+                 (long long)rows[i]);
+    PMOE_REQUIRE(rows[i] == 0 || arrays[i], "%s: null tensor (layer %lld)", what, (long long)i);
+    plan->rows = std::max(plan->rows, rows[i]);
+    total += rows[i];
+  }
+  PMOE_REQUIRE(total <= kMaxIndex, "%s: %lld rows in all", what, (long long)total);
+  plan->bpl = aux_blocks_per_layer((int)L, plan->rows);
+  return PMOE_OK;
+}
+
+int check_mask(const uint8_t* mask, int64_t mask_rows, const int64_t* rows, int64_t L, const char* what) {
+  if (mask == nullptr) return PMOE_OK;
+  for (int64_t i = 0; i < L; ++i)
+    PMOE_REQUIRE(rows[i] == mask_rows, "%s: a mask of %lld rows, but layer %lld has %lld", what, (long long)mask_rows,
+                 (long long)i, (long long)rows[i]);
+  return PMOE_OK;
+}
+
+size_t aux_bytes(int64_t L, int bpl, int64_t E) {
+  const size_t nb = (size_t)L * bpl;
+  return 2 * align_up(nb * E * 4) + 2 * align_up(nb * 4) + 2 * align_up((size_t)E * 8);
+}
+
+AuxLayers layer_table(const void* const* logits, const int64_t* rows, int64_t first, int n) {
+  AuxLayers t{};
+  for (int i = 0; i < n; ++i) { t.logits[i] = logits[first + i]; t.rows[i] = rows[first + i]; }
+  return t;
+}
+
+}  // namespace
+}  // extern "C++"
+
+PMOE_API size_t pmoe_aux_loss_forward_workspace_size(const int64_t* row_counts, int64_t L, int64_t E) {
+  if (row_counts == nullptr || L < 1 || L > 4096 || E < 1 || E > 1024) return 0;
+  int64_t most = 0;
+  for (int64_t i = 0; i < L; ++i) most = std::max(most, row_counts[i]);
+  return aux_bytes(L, aux_blocks_per_layer((int)L, most), E);
+}
+
+PMOE_API int pmoe_aux_loss_forward(const void* const* logits, const int64_t* row_counts, int64_t L, int dtype,
+                                   const uint8_t* mask, int64_t mask_rows, int64_t E, int64_t K, float aux_coef,
+                                   float z_coef, float* loss, float* load_balance, float* z_loss, int32_t* expert_counts, float* coef, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  AuxPlan plan;
+  if (int rc = check_aux(logits, row_counts, L, E, K, "aux_loss_forward", &plan)) return rc;
+  if (int rc = check_mask(mask, mask_rows, row_counts, L, "aux_loss_forward")) return rc;
+  PMOE_REQUIRE(dtype16_ok(dtype), "unknown dtype code");
+  PMOE_REQUIRE(loss && load_balance && z_loss && expert_counts && coef, "aux_loss_forward: null tensor");
+  const size_t need = aux_bytes(L, plan.bpl, E);
+  if (workspace_bytes < need || !workspace)
+    return fail(PMOE_ERR_WORKSPACE, "aux_loss_forward: workspace %zu < %zu bytes", workspace_bytes, need);
+  hipStream_t s = as_stream(stream);
+  Carver cv(workspace);
+  const size_t nb = (size_t)L * plan.bpl;
+  float* psum = cv.take<float>(nb * E);
+  int32_t* counts = cv.take<int32_t>(nb * E);
+  float* lse2 = cv.take<float>(nb);
+  int32_t* rows = cv.take<int32_t>(nb);
+  double* col_p = cv.take<double>(E);
+  int64_t* col_c = cv.take<int64_t>(E);
+  for (int64_t i = 0; i < L; i += kAuxMaxLayers) {
+    const int n = (int)std::min<int64_t>(kAuxMaxLayers, L - i);
+    const AuxLayers t = layer_table(logits, row_counts, i, n);
+    const size_t b = (size_t)i * plan.bpl;
+    hipError_t st = by_dtype16(dtype, [&](auto tp) {
+      return aux_stats<PMOE_ELEM(tp)>(t, n, mask, (int)E, (int)K, plan.bpl, psum + b * E, counts + b * E, lse2 + b,
+                                      rows + b, s);
+    });
+    PMOE_TRY(st, "aux_loss_forward");
+  }
+  return hip_status(aux_finish(psum, counts, lse2, rows, (int)L, plan.bpl, (int)E, (int)K, aux_coef, z_coef,
+                               expert_counts, col_p, col_c, AuxOut{loss, load_balance, z_loss, coef}, s),
+                    "aux_loss_forward");
+}
+
+PMOE_API size_t pmoe_aux_loss_from_stats_workspace_size(int64_t L, int64_t E) {
+  return L < 1 || E < 1 ? 0 : 2 * align_up((size_t)E * 8) + align_up(8);
+}
+
+PMOE_API int pmoe_aux_loss_from_stats(const int32_t* const* layer_counts, const float* const* prob_sums,
+                                      const float* const* lse_sq_sums, int64_t L, int64_t n, int64_t E, int64_t K,
+                                      float aux_coef, float z_coef, float* loss, float* load_balance, float* z_loss, int32_t* expert_counts, float* coef,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  PMOE_REQUIRE(L >= 1 && L <= 4096, "aux_loss_from_stats: %lld layers (1 to 4096 are supported)", (long long)L);
+  if (int rc = check_moe_dims(0, K, E, 8, 0)) return rc;
+  PMOE_REQUIRE(n >= 0 && n <= kMaxIndex, "aux_loss_from_stats: %lld rows", (long long)n);
+  PMOE_REQUIRE(layer_counts && prob_sums && lse_sq_sums && loss && load_balance && z_loss && expert_counts && coef,
+               "aux_loss_from_stats: null array");
+  for (int64_t i = 0; i < L; ++i)
+    PMOE_REQUIRE(layer_counts[i] && prob_sums[i] && lse_sq_sums[i], "aux_loss_from_stats: null tensor (layer %lld)",
+                 (long long)i);
+  const size_t need = pmoe_aux_loss_from_stats_workspace_size(L, E);
+  if (workspace_bytes < need || !workspace)
+    return fail(PMOE_ERR_WORKSPACE, "aux_loss_from_stats: workspace %zu < %zu bytes", workspace_bytes, need);
+  Carver cv(workspace);
+  double* col_p = cv.take<double>(E);
+  int64_t* col_c = cv.take<int64_t>(E);
+  double* lse2 = cv.take<double>(1);
+  for (int64_t i = 0; i < L; i += kAuxMaxLayers) {
+    const int m = (int)std::min<int64_t>(kAuxMaxLayers, L - i);
+    AuxStats st{};
+    for (int k = 0; k < m; ++k) {
+      st.counts[k] = layer_counts[i + k];
+      st.prob_sum[k] = prob_sums[i + k];
+      st.lse_sq_sum[k] = lse_sq_sums[i + k];
+    }
+    PMOE_TRY(aux_from_stats(st, m, n, (int)E, (int)K, aux_coef, z_coef, expert_counts + i * E, col_p, col_c, i == 0,
+                            i + m == L, lse2, AuxOut{loss, load_balance, z_loss, coef}, as_stream(stream)),
+             "aux_loss_from_stats");
+  }
+  return PMOE_OK;
+}
+
+PMOE_API int pmoe_aux_loss_backward(const void* const* logits, void* const* grads, const int64_t* row_counts,
+                                    int64_t L, int dtype, const uint8_t* mask, int64_t mask_rows, int64_t E,
+                                    const float* coef, const float* grad_loss, float aux_coef, float z_coef,
+                                    void* stream) {
+  AuxPlan plan;
+  if (int rc = check_aux(logits, row_counts, L, E, 1, "aux_loss_backward", &plan)) return rc;
+  if (int rc = check_mask(mask, mask_rows, row_counts, L, "aux_loss_backward")) return rc;
+  PMOE_REQUIRE(dtype16_ok(dtype), "unknown dtype code");
+  PMOE_REQUIRE(grads && coef && grad_loss, "aux_loss_backward: null tensor");
+  if (plan.rows == 0) return PMOE_OK;
+  for (int64_t i = 0; i < L; i += kAuxMaxLayers) {
+    const int n = (int)std::min<int64_t>(kAuxMaxLayers, L - i);
+    const AuxLayers t = layer_table(logits, row_counts, i, n);
+    AuxGrads g{};
+    for (int k = 0; k < n; ++k) g.grad[k] = grads[i + k];
+    hipError_t st = by_dtype16(dtype, [&](auto tp) {
+      return aux_grad<PMOE_ELEM(tp)>(t, g, n, plan.rows, mask, (int)E, coef, grad_loss, aux_coef, z_coef,
+                                     as_stream(stream));
+    });
+    PMOE_TRY(st, "aux_loss_backward");
+  }
+  return PMOE_OK;
+}
+
+// ------------------------------------------------------------- layer norm
+
+extern "C++" {
+namespace {
+
+constexpr int64_t kLnMaxRows = ((int64_t)1 << 24) - 1;  // 256 threads a row, below 2^32 a launch
+
+int check_layernorm(int64_t T, int64_t H, int x_dtype, int w_dtype, int y_dtype, const char* what) {
+  PMOE_REQUIRE(T >= 0 && H > 0 && H <= (int64_t)1 << 30, "%s: bad sizes T=%lld H=%lld", what, (long long)T,
+               (long long)H);
+  PMOE_REQUIRE(dtype16_ok(x_dtype) && dtype16_ok(w_dtype) && dtype16_ok(y_dtype), "unknown dtype code");
+  PMOE_REQUIRE(y_dtype == x_dtype || x_dtype == PMOE_F32, "%s: the output has x's type, or 16 bits beside fp32 x",
+               what);
+  if (T > kLnMaxRows)
+    return fail(PMOE_ERR_UNSUPPORTED, "%s: %lld rows > %lld", what, (long long)T, (long long)kLnMaxRows);
+  return PMOE_OK;
+}
+
+// Calls f(null pointer of x's type, null pointer of y's type) for the pairs check_layernorm admits.
+template <class F>
+hipError_t by_norm_types(int x_dtype, int y_dtype, F&& f) {
+  if (x_dtype == PMOE_BF16) return f(static_cast<bf16_t*>(nullptr), static_cast<bf16_t*>(nullptr));
+  if (x_dtype == PMOE_F16) return f(static_cast<f16_t*>(nullptr), static_cast<f16_t*>(nullptr));
+  return by_dtype16(y_dtype, [&](auto yp) { return f(static_cast<float*>(nullptr), yp); });
+}
+
+}  // namespace
+}  // extern "C++"
+
+PMOE_API int pmoe_layernorm_forward(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype,
+                                    float eps, int64_t T, int64_t H, void* out, int out_dtype, float* mean,
+                                    float* rstd, void* stream) {
+  if (int rc = check_layernorm(T, H, x_dtype, w_dtype, out_dtype, "layernorm_forward")) return rc;
+  PMOE_REQUIRE(eps >= 0.0f, "layernorm_forward: eps must be non-negative");
+  PMOE_REQUIRE((mean == nullptr) == (rstd == nullptr), "layernorm_forward: mean and rstd come together");
+  if (T == 0) return PMOE_OK;
+  PMOE_REQUIRE(x && out, "layernorm_forward: null tensor");
+  hipError_t st = by_norm_types(x_dtype, out_dtype, [&](auto xp, auto op) {
+    typedef PMOE_ELEM(xp) X;
+    typedef PMOE_ELEM(op) O;
+    return layernorm_fwd<X, O>((const X*)x, weight, bias, w_dtype, eps, T, (int)H, (O*)out, mean, rstd,
+                               as_stream(stream));
+  });
+  return hip_status(st, "layernorm_forward");
+}
+
+PMOE_API size_t pmoe_layernorm_backward_workspace_size(int64_t T, int64_t H) {
+  if (T <= 0 || T > kLnMaxRows || H <= 0 || H > (int64_t)1 << 30) return 0;
+  return align_up((size_t)2 * layernorm_bwd_blocks(T, (int)H) * layernorm_part_ld((int)H) * sizeof(float));
+}
+
+PMOE_API int pmoe_layernorm_backward(const void* grad, int grad_dtype, const void* x, int x_dtype, const void* weight,
+                                     int w_dtype, const float* mean, const float* rstd, int64_t T, int64_t H,
+                                     void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  if (int rc = check_layernorm(T, H, x_dtype, w_dtype, grad_dtype, "layernorm_backward")) return rc;
+  PMOE_REQUIRE(T == 0 || (grad && x && mean && rstd), "layernorm_backward: null tensor");
+  const bool sums = grad_weight || grad_bias;
+  if (!sums && (!grad_x || T == 0)) return PMOE_OK;
+  const size_t need = sums ? pmoe_layernorm_backward_workspace_size(T, H) : 0;
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(PMOE_ERR_WORKSPACE, "layernorm_backward: workspace %zu < %zu bytes", workspace_bytes, need);
+  PMOE_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+               "layernorm_backward: the workspace must be 16-byte aligned");
+  hipError_t st = by_norm_types(x_dtype, grad_dtype, [&](auto xp, auto gp) {
+    typedef PMOE_ELEM(xp) X;
+    typedef PMOE_ELEM(gp) G;
+    return layernorm_bwd<X, G>((const G*)grad, (const X*)x, weight, w_dtype, mean, rstd, T, (int)H, (X*)grad_x,
+                               need > 0 ? static_cast<float*>(workspace) : nullptr, grad_weight, grad_bias,
+                               as_stream(stream));
+  });
+  return hip_status(st, "layernorm_backward");
+}
+
+// --------------------------------------- activation checkpoints in 8 bits
+
+extern "C++" {
+namespace {
+
+int check_act8(int64_t R, int64_t C, int dtype, const char* what) {
+  PMOE_REQUIRE(R >= 0 && C > 0 && C <= (int64_t)1 << 30, "%s: bad sizes R=%lld C=%lld", what, (long long)R,
+               (long long)C);
+  PMOE_REQUIRE(dtype16_ok(dtype), "unknown dtype code");
+  const int64_t row = 4 * (int64_t)act8_groups((int)C);  // threads a row
+  if (R > (((int64_t)1 << 32) - 256) / row)
+    return fail(PMOE_ERR_UNSUPPORTED, "%s: %lld x %lld values exceed one launch", what, (long long)R, (long long)C);
+  return PMOE_OK;
+}
+
+int check_act8_gemm(int64_t P, int64_t E, int64_t H, int64_t I, int dtype, const char* what) {
+  if (int rc = check_moe_dims(P, 1, E, H, I)) return rc;
+  PMOE_REQUIRE(I > 0, "%s: bad I", what);
+  return check_act8(2 * P, I, dtype, what);
+}
+
+}  // namespace
+}  // extern "C++"
+
+PMOE_API int pmoe_act8_save(const void* x, int dtype, int64_t R, int64_t C, int8_t* codes, uint8_t* exps,
+                            void* stream) {
+  if (int rc = check_act8(R, C, dtype, "act8_save")) return rc;
+  if (R == 0) return PMOE_OK;
+  PMOE_REQUIRE(x && codes && exps, "act8_save: null tensor");
+  hipError_t st = by_dtype16(dtype, [&](auto tp) {
+    typedef PMOE_ELEM(tp) X;
+    return act8_save<X>((const X*)x, R, (int)C, codes, exps, as_stream(stream));
+  });
+  return hip_status(st, "act8_save");
+}
+
+PMOE_API int pmoe_act8_restore(const int8_t* codes, const uint8_t* exps, int64_t R, int64_t C, void* x, int dtype,
+                               void* stream) {
+  if (int rc = check_act8(R, C, dtype, "act8_restore")) return rc;
+  if (R == 0) return PMOE_OK;
+  PMOE_REQUIRE(x && codes && exps, "act8_restore: null tensor");
+  hipError_t st = by_dtype16(dtype, [&](auto tp) {
+    typedef PMOE_ELEM(tp) X;
+    return act8_restore<X>(codes, exps, R, (int)C, (X*)x, as_stream(stream));
+  });
+  return hip_status(st, "act8_restore");
+}
+
+PMOE_API size_t pmoe_gate_up_swiglu_act8_workspace_size(int64_t P, int64_t E, int64_t H, int64_t I, int dtype) {
+  (void)E; (void)H;
+  if (P <= 0 || I <= 0) return 0;
+  return align_up((size_t)P * 2 * I * elem_bytes(dtype));
+}
+
+PMOE_API int pmoe_gate_up_swiglu_act8(const void* x, const int32_t* row_index, const float* row_weight, int64_t x_rows,
+                                      const void* gate_up_proj, const int32_t* offs, int dtype, int64_t P, int64_t E,
+                                      int64_t H, int64_t I, int8_t* codes, uint8_t* exps, void* mid, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  if (int rc = check_act8_gemm(P, E, H, I, dtype, "gate_up_swiglu_act8")) return rc;
+  if (int rc = check_gather(row_index, x_rows, H, dtype, P, "gate_up_swiglu_act8")) return rc;
+  if (P == 0) return PMOE_OK;
+  PMOE_REQUIRE(x && gate_up_proj && offs && codes && exps && mid, "gate_up_swiglu_act8: null tensor");
+  const size_t need = pmoe_gate_up_swiglu_act8_workspace_size(P, E, H, I, dtype);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(PMOE_ERR_WORKSPACE, "gate_up_swiglu_act8: workspace %zu < %zu bytes", workspace_bytes, need);
+  if (int rc = pmoe_gate_up_swiglu(x, row_index, row_weight, x_rows, gate_up_proj, offs, dtype, P, E, H, I, workspace,
+                                   mid, stream))
+    return rc;
+  return pmoe_act8_save(workspace, dtype, 2 * P, I, codes, exps, stream);
+}
+
+PMOE_API size_t pmoe_down_proj_dgrad_act8_workspace_size(int64_t P, int64_t E, int64_t H, int64_t I, int dtype) {
+  (void)E; (void)H;
+  if (P <= 0 || I <= 0) return 0;
+  return align_up((size_t)P * 2 * I * elem_bytes(dtype)) + align_up((size_t)P * I * elem_bytes(dtype));
+}
+
+PMOE_API int pmoe_down_proj_dgrad_act8(const void* grad, const int32_t* row_index, const float* row_weight,
+                                       int64_t grad_rows, const int8_t* codes, const uint8_t* exps,
+                                       const void* down_proj, const int32_t* offs, int dtype, int64_t P, int64_t E,
+                                       int64_t H, int64_t I, void* grad_gate_up_out, void* mid, float* part,
+                                       int64_t part_ld, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_act8_gemm(P, E, H, I, dtype, "down_proj_dgrad_act8")) return rc;
+  if (int rc = check_gather(row_index, grad_rows, H, dtype, P, "down_proj_dgrad_act8")) return rc;
+  if (P == 0) return PMOE_OK;
+  PMOE_REQUIRE(grad && codes && exps && down_proj && offs && grad_gate_up_out, "down_proj_dgrad_act8: null tensor");
+  const size_t need = pmoe_down_proj_dgrad_act8_workspace_size(P, E, H, I, dtype);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(PMOE_ERR_WORKSPACE, "down_proj_dgrad_act8: workspace %zu < %zu bytes", workspace_bytes, need);
+  Carver cv(workspace);
+  char* gu = cv.take<char>((size_t)P * 2 * I * elem_bytes(dtype));
+  char* act = mid != nullptr ? static_cast<char*>(mid) : cv.take<char>((size_t)P * I * elem_bytes(dtype));
+  hipError_t st = by_dtype16(dtype, [&](auto tp) {
+    typedef PMOE_ELEM(tp) X;
+    return act8_restore_swiglu<X>(codes, exps, row_weight, P, (int)I, (X*)gu, (X*)act, as_stream(stream));
+  });
+  PMOE_TRY(st, "down_proj_dgrad_act8");
+  return pmoe_down_proj_backward(grad, row_index, row_weight, grad_rows, nullptr, gu, down_proj, offs, dtype, P, E, H,
+                                 I, grad_gate_up_out, nullptr, dtype, part, part_ld, stream);
 }
 
 }  // extern "C"

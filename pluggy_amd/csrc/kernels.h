@@ -143,6 +143,55 @@ constexpr int kRowGroup = 32;
 int rmsnorm_bwd_groups(int T_);
 hipError_t sum_row_groups(const float* partial, int rows, int n, float* tmp, hipStream_t s);
 
+// ---- layer norm (layernorm.hip). w, b: (H,) of w_code (0 fp32, 1 bf16, 2 fp16) or null; mean, rstd: (T,) fp32.
+template <typename TX, typename TO>
+hipError_t layernorm_fwd(const TX* x, const void* w, const void* b, int w_code, float eps, int64_t T_, int H, TO* out,
+                         float* mean, float* rstd, hipStream_t s);
+// gx, gw and gb may each be null; part: 2 * layernorm_bwd_blocks(T, H) rows of
+// layernorm_part_ld(H) floats, 16-byte aligned (null when neither gw nor gb is wanted).
+template <typename TX, typename TG>
+hipError_t layernorm_bwd(const TG* g, const TX* x, const void* w, int w_code, const float* mean, const float* rstd,
+                         int64_t T_, int H, TX* gx, float* part, void* gw, void* gb, hipStream_t s);
+int layernorm_bwd_blocks(int64_t T_, int H);
+int64_t layernorm_part_ld(int H);
+
+// ---- activations saved in 8 bits (act8.hip; the format: act8.h). codes (R, C)
+// int8, exps (R, groups(C)) one byte a group; of gate_up rows (P, 2I): codes (P, 2I), exps (P, 2, groups(I)).
+template <typename T>
+hipError_t act8_save(const T* x, int64_t R, int C, int8_t* codes, uint8_t* exps, hipStream_t s);
+template <typename T>
+hipError_t act8_restore(const int8_t* codes, const uint8_t* exps, int64_t R, int C, T* x, hipStream_t s);
+template <typename T>
+hipError_t act8_restore_swiglu(const int8_t* codes, const uint8_t* exps, const float* row_w, int64_t P, int I, T* gu,
+                               T* mid, hipStream_t s);
+
+// ---- the router's auxiliary loss (aux_loss.hip). Up to kAuxMaxLayers layers a launch.
+constexpr int kAuxMaxLayers = 64;
+constexpr int kAuxBlocks = 512;
+struct AuxLayers { const void* logits[kAuxMaxLayers]; int64_t rows[kAuxMaxLayers]; };
+struct AuxGrads { void* grad[kAuxMaxLayers]; };
+struct AuxStats {
+  const int32_t* counts[kAuxMaxLayers];
+  const float* prob_sum[kAuxMaxLayers];
+  const float* lse_sq_sum[kAuxMaxLayers];
+};
+struct AuxOut { float* loss; float* balance; float* z; float* f; };  // f: E + 1 floats for aux_grad (f_e and 1 / n)
+int aux_blocks_per_layer(int L, int64_t max_rows);
+// Partial sums of L * bpl blocks: psum and counts (L * bpl, E), lse2 and rows (L * bpl).
+template <typename T>
+hipError_t aux_stats(const AuxLayers& layers, int L, const uint8_t* mask, int E, int K, int bpl, float* psum,
+                     int32_t* counts, float* lse2, int32_t* rows, hipStream_t s);
+// counts (L, E); col_p, col_c: E each.
+hipError_t aux_finish(const float* psum, const int32_t* part_counts, const float* lse2, const int32_t* rows, int L,
+                      int bpl, int E, int K, float a, float z, int32_t* counts, double* col_p, int64_t* col_c,
+                      const AuxOut& out, hipStream_t s);
+hipError_t aux_from_stats(const AuxStats& st, int L, int64_t n, int E, int K, float a, float z, int32_t* counts,
+                          double* col_p, int64_t* col_c, bool first, bool last, double* lse2_sum, const AuxOut& out,
+                          hipStream_t s);
+template <typename T>
+hipError_t aux_grad(const AuxLayers& layers, const AuxGrads& grads, int L, int64_t max_rows, const uint8_t* mask,
+                    int E, const float* f, const float* dloss, float a, float z, hipStream_t s);
+
 // Chunk size (pairs) of the permutation histogram and the workspace it needs.
 constexpr int kPermuteChunk = 2048;
 // Most split-K planes of the bf16-pieces router logits GEMM (the top-k kernel

@@ -1,0 +1,122 @@
+"""Layer norm on HIP, beside the RMSNorm of ``moe_sublayer``.
+
+``layer_norm`` is ``torch.nn.functional.layer_norm`` over the last dimension,
+forward and backward, in fp32 arithmetic; ``moe_sublayer`` calls it for a block
+whose norm is a ``torch.nn.LayerNorm``. Eager calls go through one
+``torch.autograd.Function`` (or, where no gradient is wanted, straight to the
+kernel); under ``torch.compile`` they are the custom ops ``pmoe::layer_norm_fwd``
+and ``pmoe::layer_norm_bwd``, which trace without graph breaks.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+from ._lib import require_gpu
+from .moe import _empty_like_none, _refuse_capture, _stage
+
+
+def _backward(grad, x, weight, bias, mean, rstd, needs):
+    """The gradients of x, weight and bias (None where ``needs`` says so)."""
+    _refuse_capture("layer_norm_bwd")
+    dt = next((p.dtype for p in (weight, bias) if p is not None), torch.float32)
+    with _stage("layernorm_bwd"):
+        return ops.layernorm_backward(grad, x, weight, mean, rstd, dt, *needs)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, out_dtype):
+        with _stage("layernorm"):
+            out, mean, rstd = ops.layernorm_forward(x, weight, bias, eps, out_dtype)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        return (*_backward(grad.contiguous(), x, weight, bias, mean, rstd, ctx.needs_input_grad[:3]), None, None)
+
+
+@torch.library.custom_op("pmoe::layer_norm_fwd", mutates_args=(),
+                         schema="(Tensor x, Tensor? weight, Tensor? bias, float eps, ScalarType out_dtype) -> "
+                                "(Tensor, Tensor, Tensor)")
+def _layer_norm_fwd(x, weight, bias, eps, out_dtype):
+    with _stage("layernorm"):
+        return ops.layernorm_forward(x, weight, bias, eps, out_dtype)
+
+
+@_layer_norm_fwd.register_fake
+def _(x, weight, bias, eps, out_dtype):
+    f32 = torch.float32
+    return torch.empty_like(x, dtype=out_dtype), x.new_empty(x.shape[0], dtype=f32), x.new_empty(x.shape[0], dtype=f32)
+
+
+@torch.library.custom_op("pmoe::layer_norm_bwd", mutates_args=(),
+                         schema="(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor mean, Tensor rstd, "
+                                "bool[] needs) -> (Tensor, Tensor, Tensor)")
+def _layer_norm_bwd(grad, x, weight, bias, mean, rstd, needs):
+    got = _backward(grad, x, weight, bias, mean, rstd, needs)
+    return tuple(g if g is not None else _empty_like_none(x) for g in got)
+
+
+@_layer_norm_bwd.register_fake
+def _(grad, x, weight, bias, mean, rstd, needs):
+    return tuple(torch.empty_like(t) if need else _empty_like_none(x) for need, t in zip(needs, (x, weight, bias)))
+
+
+def _setup(ctx, inputs, output):
+    x, weight, bias, _eps, _out_dtype = inputs
+    _out, mean, rstd = output
+    ctx.save_for_backward(x, weight, bias, mean, rstd)
+    ctx.mark_non_differentiable(mean, rstd)
+    ctx.set_materialize_grads(False)
+
+
+def _autograd(ctx, grad, _gm, _gr):
+    if grad is None:
+        return (None,) * 5
+    x, weight, bias, mean, rstd = ctx.saved_tensors
+    needs = [bool(n) for n in ctx.needs_input_grad[:3]]
+    got = torch.ops.pmoe.layer_norm_bwd(grad.contiguous(), x, weight, bias, mean, rstd, needs)
+    return (*(g if need else None for g, need in zip(got, needs)), None, None)
+
+
+_layer_norm_fwd.register_autograd(_autograd, setup_context=_setup)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``torch.nn.functional.layer_norm(x, (H,), weight, bias, eps)`` over the last
+    dimension of ``x`` (..., H), any H, in fp32 arithmetic.
+
+    ``x``, ``weight`` and ``bias`` are fp32, bf16 or fp16; parameters of two
+    types are both taken in fp32. The result has ``x``'s type, or ``out_dtype``
+    (16 bits from fp32 ``x``: what the 16-bit products of the block read, without
+    a cast between). Unlike torch's, it does not follow autocast. Gradients reach
+    ``x`` and the parameters; a second derivative is refused, and so is a
+    backward under HIP graph capture.
+    """
+    assert x.dim() >= 1 and x.shape[-1] >= 1, "layer_norm expects (..., H)"
+    H = x.shape[-1]
+    for name, p in (("weight", weight), ("bias", bias)):
+        assert p is None or tuple(p.shape) == (H,), f"layer_norm: {name} {tuple(p.shape)}, expected ({H},)"
+    require_gpu(x, weight, bias)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    assert out_dtype == x.dtype or (x.dtype == torch.float32 and out_dtype in (torch.bfloat16, torch.float16)), (
+        f"layer_norm: {out_dtype} from {x.dtype}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        weight, bias = weight.float(), bias.float()
+    rows = x.reshape(-1, H).contiguous()
+    weight, bias = (p if p is None else p.contiguous() for p in (weight, bias))
+    if torch.compiler.is_compiling():
+        out = torch.ops.pmoe.layer_norm_fwd(rows, weight, bias, float(eps), out_dtype)[0]
+    elif torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rows, weight, bias)):
+        out = _LayerNorm.apply(rows, weight, bias, float(eps), out_dtype)
+    else:
+        with _stage("layernorm"):
+            out = ops.layernorm_forward(rows, weight, bias, float(eps), out_dtype, stats=False)[0]
+    return out.reshape(x.shape)

@@ -420,8 +420,20 @@ def router_topk(hidden: torch.Tensor, weight: torch.Tensor, top_k: int, norm_top
 # -------------------------------------------------------------- expert FFN
 
 
-def _ffn_forward(hidden, top_indices, top_weights, gate_up_proj, down_proj):
-    """-> out and what the backward reads: offs, inv_pos, sorted_token, sorted_w, gu, mid.
+def _gate_up(hidden, gate_up_proj, offs, sorted_token, sorted_w, act8):
+    """-> mid and the pair that the backward keeps: gu and mid, or with act8 the 8-bit checkpoint of
+    gu (codes, exps), from which the backward computes mid again."""
+    with _stage("gate_up_fwd"):
+        if act8:
+            codes, exps, mid = ops.gate_up_swiglu_act8(hidden, gate_up_proj, offs, sorted_token, sorted_w)
+            return mid, codes, exps
+        gu, mid = ops.gate_up_swiglu(hidden, gate_up_proj, offs, sorted_token, sorted_w)
+        return mid, gu, mid
+
+
+def _ffn_forward(hidden, top_indices, top_weights, gate_up_proj, down_proj, act8=False):
+    """-> out and what the backward reads: offs, inv_pos, sorted_token, sorted_w, gu, mid (with act8:
+    codes, exps in place of the last two).
 
     The expert-sorted copy of the hidden rows (moe.py:104) is never built: the
     gate_up GEMM gathers row sorted_token[p] of ``hidden`` in its operand loads,
@@ -432,21 +444,27 @@ def _ffn_forward(hidden, top_indices, top_weights, gate_up_proj, down_proj):
     K = top_indices.shape[1]
     with _stage("permute"):
         _, offs, _sorted_pair, inv_pos, sorted_token, sorted_w = ops.permute_rows(top_indices, top_weights, E)
-    with _stage("gate_up_fwd"):
-        gu, mid = ops.gate_up_swiglu(hidden, gate_up_proj, offs, sorted_token, sorted_w)
+    mid, gu, kept = _gate_up(hidden, gate_up_proj, offs, sorted_token, sorted_w, act8)
     with _stage("down_fwd"):
         y = ops.down_proj(mid, down_proj, offs)
     with _stage("combine"):
         out = ops.combine(y, None, inv_pos, K)
-    return out, offs, inv_pos, sorted_token, sorted_w, gu, mid
+    return out, offs, inv_pos, sorted_token, sorted_w, gu, kept
 
 
-def _ffn_fake_saved(hidden, K, E, I):
+def _fake_gate_up(x, P, I, act8):
+    """The pair that ``_gate_up`` keeps."""
+    if act8:
+        return x.new_empty(P, 2 * I, dtype=torch.int8), x.new_empty(P, 2, ops.act8_groups(I), dtype=torch.uint8)
+    return x.new_empty(P, 2 * I), x.new_empty(P, I)
+
+
+def _ffn_fake_saved(hidden, K, E, I, act8=False):
     T, H = hidden.shape
     P = T * K
     i32 = torch.int32
     return (hidden.new_empty(E, dtype=i32), hidden.new_empty(P, dtype=i32), hidden.new_empty(P, dtype=i32),
-            hidden.new_empty(P, dtype=torch.float32), hidden.new_empty(P, 2 * I), hidden.new_empty(P, I))
+            hidden.new_empty(P, dtype=torch.float32), *_fake_gate_up(hidden, P, I, act8))
 
 
 # Check caller-supplied expert ids before routing (moe_expert_ffn). The
@@ -465,21 +483,22 @@ def _check_expert_ids(top_indices: torch.Tensor, num_experts: int) -> None:
 
 @torch.library.custom_op("pmoe::expert_ffn_fwd", mutates_args=(),
                          schema="(Tensor hidden, Tensor top_indices, Tensor top_weights, Tensor gate_up_proj, "
-                                "Tensor down_proj, Tensor? gate_up_master=None, Tensor? down_master=None) -> "
-                                "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)")
+                                "Tensor down_proj, Tensor? gate_up_master=None, Tensor? down_master=None, "
+                                "bool act8=False) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)")
 def _expert_ffn_fwd(hidden, top_indices, top_weights, gate_up_proj, down_proj, gate_up_master=None,
-                    down_master=None):
+                    down_master=None, act8=False):
     """The masters, when given, are the differentiable fp32 weights whose bf16
-    copies gate_up_proj / down_proj are; the forward does not read them."""
+    copies gate_up_proj / down_proj are; the forward does not read them. act8:
+    keep the pre-activations in 8 bits (``_gate_up``)."""
     if VALIDATE_EXPERT_IDS:
         _check_expert_ids(top_indices, gate_up_proj.shape[0])
-    return _ffn_forward(hidden, top_indices, top_weights, gate_up_proj, down_proj)
+    return _ffn_forward(hidden, top_indices, top_weights, gate_up_proj, down_proj, act8)
 
 
 @_expert_ffn_fwd.register_fake
-def _(hidden, top_indices, top_weights, gate_up_proj, down_proj, gate_up_master=None, down_master=None):
+def _(hidden, top_indices, top_weights, gate_up_proj, down_proj, gate_up_master=None, down_master=None, act8=False):
     E, I2 = gate_up_proj.shape[0], gate_up_proj.shape[1]
-    return (torch.empty_like(hidden),) + _ffn_fake_saved(hidden, top_indices.shape[1], E, I2 // 2)
+    return (torch.empty_like(hidden),) + _ffn_fake_saved(hidden, top_indices.shape[1], E, I2 // 2, act8)
 
 
 @torch.library.custom_op("pmoe::expert_bwd_dgrad", mutates_args=(),
@@ -505,6 +524,47 @@ def _(grad_out, down_proj, offs, inv_pos, sorted_token, sorted_w, gu, top_k, nee
     P = sorted_token.shape[0]
     return (gu.new_empty(P, gu.shape[1]),
             grad_out.new_empty(P // top_k, top_k, dtype=torch.float32) if need_top_w else _empty_like_none(sorted_w))
+
+
+@torch.library.custom_op("pmoe::expert_bwd_dgrad_act8", mutates_args=(),
+                         schema="(Tensor grad_out, Tensor down_proj, Tensor offs, Tensor inv_pos, Tensor sorted_token, "
+                                "Tensor sorted_w, Tensor codes, Tensor exps, int top_k, bool need_top_w, "
+                                "bool need_mid) -> (Tensor, Tensor, Tensor)")
+def _expert_bwd_dgrad_act8(grad_out, down_proj, offs, inv_pos, sorted_token, sorted_w, codes, exps, top_k, need_top_w,
+                           need_mid):
+    """``expert_bwd_dgrad`` from the 8-bit checkpoint of the pre-activations: ->
+    grad_gate_up_out, the routing weights' gradient and mid, computed again for
+    the down weight gradient (each of the last two an empty stand-in unless
+    needed)."""
+    _refuse_capture("expert_bwd_dgrad_act8")
+    with _stage("down_dgrad"):
+        g_gu, mid, part = ops.down_proj_dgrad_act8(grad_out, codes, exps, down_proj, offs, sorted_token, sorted_w,
+                                                   need_part=need_top_w, need_mid=need_mid)
+    mid = mid if mid is not None else _empty_like_none(grad_out)
+    if not need_top_w:
+        return g_gu, _empty_like_none(sorted_w), mid
+    with _stage("pair_wgrad"):
+        return g_gu, ops.pair_weight_grad(part, inv_pos, top_k), mid
+
+
+@_expert_bwd_dgrad_act8.register_fake
+def _(grad_out, down_proj, offs, inv_pos, sorted_token, sorted_w, codes, exps, top_k, need_top_w, need_mid):
+    P, I = sorted_token.shape[0], down_proj.shape[2]
+    f32 = torch.float32
+    return (grad_out.new_empty(P, 2 * I),
+            grad_out.new_empty(P // top_k, top_k, dtype=f32) if need_top_w else _empty_like_none(sorted_w),
+            grad_out.new_empty(P, I) if need_mid else _empty_like_none(grad_out))
+
+
+def _dgrad(act8, grad_out, down, offs, inv_pos, sorted_token, sorted_w, gu, kept, top_k, need_top_w, need_mid):
+    """The down dgrad op for the pair that ``_gate_up`` kept: -> grad_gate_up_out, the routing weights'
+    gradient (or its stand-in), mid."""
+    if act8:
+        return torch.ops.pmoe.expert_bwd_dgrad_act8(grad_out, down, offs, inv_pos, sorted_token, sorted_w, gu, kept,
+                                                    top_k, need_top_w, need_mid)
+    g_gu, g_w = torch.ops.pmoe.expert_bwd_dgrad(grad_out, down, offs, inv_pos, sorted_token, sorted_w, gu, top_k,
+                                                need_top_w)
+    return g_gu, g_w, kept
 
 
 def _expert_gemms_backward(g_gu, grad_out, hidden, gate_up, down, offs, sorted_token, mid, need_rows, need_gu,
@@ -570,7 +630,8 @@ def _(g_gu, grad_out, hidden, gate_up, down, offs, inv_pos, sorted_token, mid, g
 
 
 def _ffn_setup(ctx, inputs, output):
-    hidden, top_indices, top_weights, gate_up_proj, down_proj, gate_up_master, down_master = inputs
+    hidden, top_indices, top_weights, gate_up_proj, down_proj, gate_up_master, down_master, act8 = inputs
+    ctx.act8 = bool(act8)
     ctx.f32_wgrads = _f32_wgrads(gate_up_master, down_master)
     out, offs, inv_pos, sorted_token, sorted_w, gu, mid = output
     ctx.save_for_backward(hidden, gate_up_proj, down_proj, offs, inv_pos, sorted_token, sorted_w, gu, mid)
@@ -582,18 +643,18 @@ def _ffn_setup(ctx, inputs, output):
 
 def _ffn_backward(ctx, grad_out, *_saved_grads):
     if grad_out is None:
-        return (None,) * 7
+        return (None,) * 8
     hidden, gate_up, down, offs, inv_pos, sorted_token, sorted_w, gu, mid = ctx.saved_tensors
     K = ctx.top_k
-    need = _needs(ctx, 7)  # hidden, indices, weights, gate_up, down, gate_up_master, down_master
+    need = _needs(ctx, 8)  # hidden, indices, weights, gate_up, down, gate_up_master, down_master, act8
     need_gu, need_dn = need[3] or need[5], need[4] or need[6]
     if not (need[0] or need[2] or need_gu or need_dn):
-        return (None,) * 7
+        return (None,) * 8
     grad_out = grad_out.contiguous()
     if grad_out.dtype != hidden.dtype:
         grad_out = grad_out.to(hidden.dtype)
-    g_gu, g_w = torch.ops.pmoe.expert_bwd_dgrad(grad_out, down, offs, inv_pos, sorted_token, sorted_w, gu, K,
-                                                bool(need[2]))
+    g_gu, g_w, mid = _dgrad(ctx.act8, grad_out, down, offs, inv_pos, sorted_token, sorted_w, gu, mid, K,
+                            bool(need[2]), bool(need_dn))
     g_hidden = g_gu_w = g_dn_w = None
     if need[0] or need_gu or need_dn:
         g_hidden, g_gu_w, g_dn_w = torch.ops.pmoe.expert_bwd(g_gu, grad_out, hidden, gate_up, down, offs, inv_pos,
@@ -603,7 +664,7 @@ def _ffn_backward(ctx, grad_out, *_saved_grads):
         g_hidden, g_gu_w, g_dn_w = (_none_if_empty(t) for t in (g_hidden, g_gu_w, g_dn_w))
     g_w = g_w.to(ctx.tw_dtype) if need[2] else None
     return (g_hidden if need[0] else None, None, g_w, g_gu_w if need[3] else None, g_dn_w if need[4] else None,
-            g_gu_w if need[5] else None, g_dn_w if need[6] else None)
+            g_gu_w if need[5] else None, g_dn_w if need[6] else None, None)
 
 
 _expert_ffn_fwd.register_autograd(_ffn_backward, setup_context=_ffn_setup)
@@ -615,11 +676,11 @@ _expert_ffn_fwd.register_autograd(_ffn_backward, setup_context=_ffn_setup)
 @torch.library.custom_op("pmoe::sparse_moe_fwd", mutates_args=(),
                          schema="(Tensor x, Tensor router_weight, Tensor gate_up_proj, Tensor down_proj, int top_k, "
                                 "bool norm_topk_prob, Tensor? logit_bias, Tensor? gate_up_master=None, "
-                                "Tensor? down_master=None, Tensor? router_pieces=None) -> (Tensor, Tensor, Tensor, "
-                                "Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, "
-                                "Tensor)")
+                                "Tensor? down_master=None, Tensor? router_pieces=None, bool act8=False) -> "
+                                "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, "
+                                "Tensor, Tensor, Tensor, Tensor)")
 def _sparse_moe_fwd(x, router_weight, gate_up_proj, down_proj, top_k, norm_topk_prob, logit_bias,
-                    gate_up_master=None, down_master=None, router_pieces=None):
+                    gate_up_master=None, down_master=None, router_pieces=None, act8=False):
     """Router + dropless experts (Qwen3MoeSparseMLP.forward) as one op.
 
     -> out, router_logits, counts, prob_sum, lse_sq_sum, then what the backward
@@ -627,31 +688,33 @@ def _sparse_moe_fwd(x, router_weight, gate_up_proj, down_proj, top_k, norm_topk_
     mid. The masters, when given, are the differentiable fp32 weights whose
     bf16 copies gate_up_proj / down_proj are (their gradients are written in
     fp32). router_pieces: the router weight's bf16 pieces (``_router_pieces``),
-    reused by the backward, or None.
+    reused by the backward, or None. act8: codes and exps of gu's 8-bit
+    checkpoint in place of gu and mid.
     """
     with _stage("router_fwd"):
         logits, top_w, top_i, top_w32, counts, psum, lse2 = ops.router_forward(
             _router_x(x, router_weight), router_weight, top_k, norm_topk_prob, logit_bias, tw_dtype=x.dtype,
             pieces=router_pieces)
-    out, offs, inv_pos, stok, sw, gu, mid = _ffn_forward(x, top_i, top_w, gate_up_proj, down_proj)
+    out, offs, inv_pos, stok, sw, gu, mid = _ffn_forward(x, top_i, top_w, gate_up_proj, down_proj, act8)
     return out, logits, counts, psum, lse2, top_i, top_w32, top_w, offs, inv_pos, stok, sw, gu, mid
 
 
 @_sparse_moe_fwd.register_fake
 def _(x, router_weight, gate_up_proj, down_proj, top_k, norm_topk_prob, logit_bias, gate_up_master=None,
-      down_master=None, router_pieces=None):
+      down_master=None, router_pieces=None, act8=False):
     T, E, K = x.shape[0], router_weight.shape[0], top_k
     I = gate_up_proj.shape[1] // 2
     f32 = torch.float32
     return ((torch.empty_like(x), x.new_empty(T, E, dtype=f32), x.new_empty(E, dtype=torch.int32),
              x.new_empty(E, dtype=f32), x.new_empty(1, dtype=f32), x.new_empty(T, K, dtype=torch.int64),
              x.new_empty(T, K, dtype=f32), x.new_empty(T, K))
-            + _ffn_fake_saved(x, K, E, I))
+            + _ffn_fake_saved(x, K, E, I, act8))
 
 
 def _sparse_setup(ctx, inputs, output):
     (x, router_weight, gate_up_proj, down_proj, top_k, norm_topk_prob, logit_bias, gu_master, dn_master,
-     router_pieces) = inputs
+     router_pieces, act8) = inputs
+    ctx.act8 = bool(act8)
     (out, logits, counts, psum, lse2, top_i, top_w32, top_w, offs, inv_pos, stok, sw, gu, mid) = output
     ctx.f32_wgrads = _f32_wgrads(gu_master, dn_master)
     ctx.save_for_backward(x, router_weight, logits, top_i, top_w32, gate_up_proj, down_proj, offs, inv_pos, stok,
@@ -668,21 +731,21 @@ def _sparse_backward(ctx, g_out, g_logits, *_rest):
     backward, so the two input gradients are never summed by a separate pass."""
     (x, rw, logits, top_i, top_w32, gate_up, down, offs, inv_pos, stok, sw, gu, mid, pieces) = ctx.saved_tensors
     T, K = ctx.dims
-    # x, router_weight, gate_up, down, top_k, norm, bias, gate_up_master, down_master, router_pieces
-    need = _needs(ctx, 10)
+    # x, router_weight, gate_up, down, top_k, norm, bias, gate_up_master, down_master, router_pieces, act8
+    need = _needs(ctx, 11)
     need_gu, need_dn = need[2] or need[7], need[3] or need[8]
     if g_out is None and g_logits is None:
-        return (None,) * 10
+        return (None,) * 11
     if g_logits is not None:
         g_logits = g_logits.float().contiguous()
     g_x = g_rw = g_gu_w = g_dn_w = None
     g_gu = g_tw = None
     if g_out is not None:
         g_out = g_out.contiguous()
-        if g_out.dtype != gu.dtype:
-            g_out = g_out.to(gu.dtype)
-        g_gu, g_tw = torch.ops.pmoe.expert_bwd_dgrad(g_out, down, offs, inv_pos, stok, sw, gu, K,
-                                                     bool(need[0] or need[1]))
+        if g_out.dtype != down.dtype:
+            g_out = g_out.to(down.dtype)
+        g_gu, g_tw, mid = _dgrad(ctx.act8, g_out, down, offs, inv_pos, stok, sw, gu, mid, K,
+                                 bool(need[0] or need[1]), bool(need_dn))
         g_tw = _none_if_empty(g_tw)
     gx_router = None
     if need[0] or need[1]:
@@ -700,21 +763,27 @@ def _sparse_backward(ctx, g_out, g_logits, *_rest):
         g_x = gx_router
     return ((g_x if need[0] else None), (g_rw if need[1] else None), g_gu_w if need[2] else None,
             g_dn_w if need[3] else None, None, None, None, g_gu_w if need[7] else None, g_dn_w if need[8] else None,
-            None)
+            None, None)
 
 
 _sparse_moe_fwd.register_autograd(_sparse_backward, setup_context=_sparse_setup)
 
 
+def _act8(checkpoint_8bit: bool) -> bool:
+    """Whether the op keeps an 8-bit checkpoint: asked for, and a backward can follow."""
+    return bool(checkpoint_8bit) and torch.is_grad_enabled()
+
+
 def sparse_moe_block(hidden: torch.Tensor, router_weight: torch.Tensor, gate_up_proj: torch.Tensor,
                      down_proj: torch.Tensor, top_k: int, norm_topk_prob: bool = True,
-                     logit_bias: torch.Tensor | None = None):
+                     logit_bias: torch.Tensor | None = None, *, checkpoint_8bit: bool = False):
     """Router + experts of ``Qwen3MoeSparseMLP.forward`` (qwen3_moe.py:233-239) on HIP.
 
     ``hidden`` (T, H). Returns ``(out (T,H), router_logits (T,E) fp32,
     RouterStats)``; the logits carry the gradient of any aux loss. Same
     arithmetic as ``router_topk`` followed by ``moe_expert_ffn``, including
     their bf16 operands under CUDA autocast (``out`` keeps ``hidden.dtype``).
+    ``checkpoint_8bit`` as in ``moe_expert_ffn``.
     """
     assert hidden.dim() == 2 and router_weight.dim() == 2 and router_weight.shape[1] == hidden.shape[1]
     assert gate_up_proj.dim() == 3 and down_proj.dim() == 3
@@ -732,7 +801,8 @@ def sparse_moe_block(hidden: torch.Tensor, router_weight: torch.Tensor, gate_up_
         logit_bias = logit_bias.float().contiguous()
     pieces = _router_pieces(dt, rw, router_weight)
     out, logits, counts, psum, lse2 = torch.ops.pmoe.sparse_moe_fwd(x, rw, gu, dn, int(top_k), bool(norm_topk_prob),
-                                                                     logit_bias, gu_master, dn_master, pieces)[:5]
+                                                                     logit_bias, gu_master, dn_master, pieces,
+                                                                     _act8(checkpoint_8bit))[:5]
     return out[:, :H].to(hidden.dtype), logits, RouterStats(counts, psum, lse2, T)
 
 
@@ -744,6 +814,7 @@ def moe_expert_ffn(
     down_proj: torch.Tensor,     # (E, H, I)
     *,
     use_grouped_mm: bool | None = None,
+    checkpoint_8bit: bool = False,
 ) -> torch.Tensor:
     """Dropless top-k expert FFN on MI355X (drop-in for moe.py:127-168).
 
@@ -752,6 +823,12 @@ def moe_expert_ffn(
     reference does (moe.py:110-112), and to bf16 under CUDA autocast, with the
     output in ``hidden.dtype``. The permutation, both grouped GEMMs and the
     fp32-accumulating combine run as HIP kernels; there is no CPU path.
+
+    With ``checkpoint_8bit`` the backward keeps the gate and up pre-activations
+    in 8 bits (``ops.act8_save``'s format) and computes the activation again
+    from them: 2 I (1 + 1/32) bytes a pair instead of 6 I at 16 bits. The output
+    is the same, bit for bit; the gradients are those of pre-activations that are
+    each off by at most a / 127, a the largest of its 32 columns' magnitudes.
     """
     assert hidden.dim() == 2
     assert top_indices.shape == top_weights.shape
@@ -767,7 +844,7 @@ def moe_expert_ffn(
     tw = top_weights if top_weights.dtype in (torch.float32, torch.bfloat16, torch.float16) else top_weights.float()
     out = torch.ops.pmoe.expert_ffn_fwd(_pad_last(hidden.to(dt), Hp).contiguous(),
                                         top_indices.to(torch.int64).contiguous(), tw.contiguous(), gu, dn,
-                                        gu_master, dn_master)[0]
+                                        gu_master, dn_master, _act8(checkpoint_8bit))[0]
     return out[:, :H].to(hidden.dtype)
 
 
@@ -777,11 +854,11 @@ def moe_expert_ffn(
 @torch.library.custom_op("pmoe::moe_sublayer_fwd", mutates_args=(),
                          schema="(Tensor x, Tensor norm_weight, float eps, Tensor router_weight, Tensor gate_up_proj, "
                                 "Tensor down_proj, int top_k, bool norm_topk_prob, Tensor? logit_bias, "
-                                "Tensor? gate_up_master=None, Tensor? down_master=None, Tensor? router_pieces=None) "
-                                "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, "
+                                "Tensor? gate_up_master=None, Tensor? down_master=None, Tensor? router_pieces=None, "
+                                "bool act8=False) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, "
                                 "Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)")
 def _moe_sublayer_fwd(x, norm_weight, eps, router_weight, gate_up_proj, down_proj, top_k, norm_topk_prob,
-                      logit_bias, gate_up_master=None, down_master=None, router_pieces=None):
+                      logit_bias, gate_up_master=None, down_master=None, router_pieces=None, act8=False):
     """x + SparseMLP(RMSNorm(x)) with the norm and the residual add in the row kernels.
 
     The kernels compute in gate_up_proj's dtype; x is the residual stream (its
@@ -790,6 +867,7 @@ def _moe_sublayer_fwd(x, norm_weight, eps, router_weight, gate_up_proj, down_pro
     sorted_token, sorted_w, gu, mid. The masters, when given, are the
     differentiable fp32 weights whose bf16 copies gate_up_proj / down_proj are;
     router_pieces, the router weight's bf16 pieces (``_router_pieces``) or None.
+    act8: codes and exps of gu's 8-bit checkpoint in place of gu and mid.
     """
     with _stage("rmsnorm"):
         normed, rstd = ops.rmsnorm_forward(x, norm_weight, eps, gate_up_proj.dtype)
@@ -798,18 +876,17 @@ def _moe_sublayer_fwd(x, norm_weight, eps, router_weight, gate_up_proj, down_pro
             normed, router_weight, top_k, norm_topk_prob, logit_bias, pieces=router_pieces)
     with _stage("permute"):
         _, offs, _sorted_pair, inv_pos, stok, sw = ops.permute_rows(top_i, top_w, gate_up_proj.shape[0])
-    with _stage("gate_up_fwd"):
-        gu, mid = ops.gate_up_swiglu(normed, gate_up_proj, offs, stok, sw)
+    mid, gu, kept = _gate_up(normed, gate_up_proj, offs, stok, sw, act8)
     with _stage("down_fwd"):
         y = ops.down_proj(mid, down_proj, offs)
     with _stage("combine"):
         out = ops.combine_residual(y, None, inv_pos, x, top_k)
-    return out, logits, counts, psum, lse2, normed, rstd, top_i, top_w32, top_w, offs, inv_pos, stok, sw, gu, mid
+    return out, logits, counts, psum, lse2, normed, rstd, top_i, top_w32, top_w, offs, inv_pos, stok, sw, gu, kept
 
 
 @_moe_sublayer_fwd.register_fake
 def _(x, norm_weight, eps, router_weight, gate_up_proj, down_proj, top_k, norm_topk_prob, logit_bias,
-      gate_up_master=None, down_master=None, router_pieces=None):
+      gate_up_master=None, down_master=None, router_pieces=None, act8=False):
     T, H = x.shape
     E, K, I = router_weight.shape[0], top_k, gate_up_proj.shape[1] // 2
     cdt = gate_up_proj.dtype
@@ -819,7 +896,7 @@ def _(x, norm_weight, eps, router_weight, gate_up_proj, down_proj, top_k, norm_t
             x.new_empty(1, dtype=f32), x.new_empty(T, H, dtype=cdt), x.new_empty(T, dtype=f32),
             x.new_empty(T, K, dtype=torch.int64), x.new_empty(T, K, dtype=f32), x.new_empty(T, K, dtype=cdt),
             x.new_empty(E, dtype=i32), x.new_empty(P, dtype=i32), x.new_empty(P, dtype=i32),
-            x.new_empty(P, dtype=f32), x.new_empty(P, 2 * I, dtype=cdt), x.new_empty(P, I, dtype=cdt))
+            x.new_empty(P, dtype=f32), *_fake_gate_up(gate_up_proj, P, I, act8))
 
 
 @torch.library.custom_op("pmoe::sublayer_bwd", mutates_args=(),
@@ -867,7 +944,8 @@ def _(g_gu, grad_out_c, normed, gate_up, down, offs, inv_pos, sorted_token, mid,
 
 def _sublayer_setup(ctx, inputs, output):
     (x, norm_weight, eps, router_weight, gate_up_proj, down_proj, top_k, norm_topk_prob, logit_bias, gu_master,
-     dn_master, router_pieces) = inputs
+     dn_master, router_pieces, act8) = inputs
+    ctx.act8 = bool(act8)
     ctx.f32_wgrads = _f32_wgrads(gu_master, dn_master)
     (out, logits, counts, psum, lse2, normed, rstd, top_i, top_w32, top_w, offs, inv_pos, stok, sw, gu,
      mid) = output
@@ -887,10 +965,10 @@ def _sublayer_backward(ctx, g_out, g_logits, *_rest):
     (x, nw, rstd, normed, rw, logits, top_i, top_w32, gate_up, down, offs, inv_pos, stok, sw, gu,
      mid, pieces) = ctx.saved_tensors
     # x, norm_weight, eps, router_weight, gate_up, down, top_k, norm, bias, gate_up_master, down_master,
-    # router_pieces
-    need = _needs(ctx, 12)
+    # router_pieces, act8
+    need = _needs(ctx, 13)
     need_gu, need_dn = need[4] or need[9], need[5] or need[10]
-    nones = (None,) * 12
+    nones = (None,) * 13
     if g_out is None and g_logits is None:
         return nones
     if g_logits is not None:
@@ -899,9 +977,9 @@ def _sublayer_backward(ctx, g_out, g_logits, *_rest):
     if g_out is not None:
         g_out = g_out.contiguous()
         # the expert GEMMs gather rows of the output gradient in the compute dtype
-        g_out_c = g_out if g_out.dtype == gu.dtype else g_out.to(gu.dtype)
-        g_gu, g_tw = torch.ops.pmoe.expert_bwd_dgrad(g_out_c, down, offs, inv_pos, stok, sw, gu, ctx.top_k,
-                                                     bool(need[0] or need[1] or need[3]))
+        g_out_c = g_out if g_out.dtype == down.dtype else g_out.to(down.dtype)
+        g_gu, g_tw, mid = _dgrad(ctx.act8, g_out_c, down, offs, inv_pos, stok, sw, gu, mid, ctx.top_k,
+                                 bool(need[0] or need[1] or need[3]), bool(need_dn))
         g_tw = _none_if_empty(g_tw)
     gx_router = g_rw = None
     if need[0] or need[1] or need[3]:
@@ -917,13 +995,13 @@ def _sublayer_backward(ctx, g_out, g_logits, *_rest):
         g_x, g_nw, g_gu_w, g_dn_w = (_none_if_empty(t) for t in (g_x, g_nw, g_gu_w, g_dn_w))
     return (g_x if need[0] else None, g_nw if need[1] else None, None, g_rw if need[3] else None,
             g_gu_w if need[4] else None, g_dn_w if need[5] else None, None, None, None, g_gu_w if need[9] else None,
-            g_dn_w if need[10] else None, None)
+            g_dn_w if need[10] else None, None, None)
 
 
 _moe_sublayer_fwd.register_autograd(_sublayer_backward, setup_context=_sublayer_setup)
 
 
-def moe_sublayer(x: torch.Tensor, norm: torch.nn.RMSNorm, mlp) -> torch.Tensor:
+def moe_sublayer(x: torch.Tensor, norm: torch.nn.RMSNorm | torch.nn.LayerNorm, mlp) -> torch.Tensor:
     """``x + mlp(norm(x))`` — the MoE half of ``Qwen3MoeTransformerBlock.forward``
     (qwen3_moe.py:281) — with the RMSNorm and the residual add fused into the
     block's row kernels.
@@ -937,9 +1015,21 @@ def moe_sublayer(x: torch.Tensor, norm: torch.nn.RMSNorm, mlp) -> torch.Tensor:
     first, as ``moe_expert_ffn``). Same value as
     ``x + mlp(norm(x))`` up to the rounding of the normed rows and of the MLP
     output, which this path does not round to the compute dtype before the add.
+    ``mlp.experts.checkpoint_8bit`` as in ``moe_expert_ffn``.
+
+    A block whose ``norm`` is a ``torch.nn.LayerNorm`` runs ``layer_norm`` into
+    the compute dtype and the MLP on its result; the residual is then added by
+    torch.
     """
     B, S, H = x.shape
     require_gpu(x)
+    if isinstance(norm, torch.nn.LayerNorm):
+        assert tuple(norm.normalized_shape) == (H,)
+        from .layernorm import layer_norm
+
+        cdt = _compute_dtype(x)
+        out_dtype = cdt if x.dtype == torch.float32 else x.dtype
+        return x + mlp(layer_norm(x, norm.weight, norm.bias, norm.eps, out_dtype))
     assert isinstance(norm, torch.nn.RMSNorm) and tuple(norm.normalized_shape) == (H,) and norm.weight is not None
     I = mlp.experts.gate_up_proj.shape[1] // 2
     if (H > 16384 or H % 8 or I % 8 or x.dtype not in (torch.float32, torch.bfloat16)
@@ -961,7 +1051,8 @@ def moe_sublayer(x: torch.Tensor, norm: torch.nn.RMSNorm, mlp) -> torch.Tensor:
     bias = r.logit_bias.float().contiguous() if r.logit_bias is not None else None
     out, logits, counts, psum, lse2 = torch.ops.pmoe.moe_sublayer_fwd(
         flat, nw.contiguous(), float(eps), rw, gu, dn, int(r.top_k), bool(r.norm_topk_prob), bias,
-        gu_master, dn_master, _router_pieces(cdt, rw, r.weight))[:5]
+        gu_master, dn_master, _router_pieces(cdt, rw, r.weight),
+        _act8(getattr(mlp.experts, "checkpoint_8bit", False)))[:5]
     r.last_stats = RouterStats(counts, psum, lse2, flat.shape[0])
     mlp.last_router_logits = logits
     return out.reshape(B, S, H)

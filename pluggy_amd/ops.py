@@ -7,9 +7,11 @@ freshly allocated on the input's device and stream.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from ._lib import PMOE_BF16X3, call, dtype_code, ptr, require_gpu, size, stream_of, workspace
+from ._lib import PMOE_BF16X3, call, dtype_code, on_device, ptr, require_gpu, size, stream_of, workspace
 
 
 def _dims(gate_up_proj: torch.Tensor):
@@ -342,3 +344,195 @@ def dispatch_rmsnorm_backward(grad_x_perm, inv_pos, grad_normed_add, x, weight, 
          ptr(x), dtype_code(x.dtype), ptr(weight), ptr(rstd), ptr(grad_residual), T, top_k, H, ptr(gx), ptr(gw),
          dtype_code(weight_dtype), ptr(ws), ws.numel(), stream_of(x))
     return gx, gw
+
+
+# ------------------------------------------------------------------ layer norm
+
+
+def layernorm_forward(x, weight, bias, eps: float, out_dtype, stats: bool = True):
+    """torch.nn.LayerNorm over the rows of x (T,H) in fp32 arithmetic -> out (T,H) out_dtype, mean and
+    rstd (T,) fp32 (None without ``stats``). weight and bias (H,), one dtype, or None."""
+    require_gpu(x, weight, bias)
+    T, H = x.shape
+    assert x.is_contiguous() and all(p is None or (p.is_contiguous() and p.shape == (H,)) for p in (weight, bias))
+    assert weight is None or bias is None or weight.dtype == bias.dtype
+    wdt = next((p.dtype for p in (weight, bias) if p is not None), torch.float32)
+    out = torch.empty(T, H, dtype=out_dtype, device=x.device)
+    mean, rstd = (torch.empty(T, dtype=torch.float32, device=x.device) if stats else None for _ in range(2))
+    with on_device(x):
+        call("pmoe_layernorm_forward", ptr(x), dtype_code(x.dtype), ptr(weight), ptr(bias), dtype_code(wdt),
+             float(eps), T, H, ptr(out), dtype_code(out_dtype), ptr(mean), ptr(rstd), stream_of(x))
+    return out, mean, rstd
+
+
+def layernorm_backward(grad, x, weight, mean, rstd, weight_dtype=torch.float32, need_x: bool = True,
+                       need_weight: bool = True, need_bias: bool = True):
+    """-> grad_x (x.dtype), grad_weight and grad_bias (weight_dtype, ``weight``'s own when it is given);
+    None where not needed. grad has the forward's out_dtype."""
+    require_gpu(grad, x, weight, mean, rstd)
+    T, H = x.shape
+    assert grad.shape == x.shape and grad.is_contiguous() and x.is_contiguous()
+    assert weight is None or weight.dtype == weight_dtype
+    dev = x.device
+    gx = torch.empty_like(x) if need_x else None
+    gw = torch.empty(H, dtype=weight_dtype, device=dev) if need_weight else None
+    gb = torch.empty(H, dtype=weight_dtype, device=dev) if need_bias else None
+    ws = workspace(size("pmoe_layernorm_backward_workspace_size", T, H) if need_weight or need_bias else 0, dev)
+    with on_device(x):
+        call("pmoe_layernorm_backward", ptr(grad), dtype_code(grad.dtype), ptr(x), dtype_code(x.dtype), ptr(weight),
+             dtype_code(weight_dtype), ptr(mean), ptr(rstd), T, H, ptr(gx), ptr(gw), ptr(gb), ptr(ws), ws.numel(),
+             stream_of(x))
+    return gx, gw, gb
+
+
+# ------------------------------------------------------ router auxiliary loss
+
+
+def _pointers(tensors):
+    """A host array of the tensors' device pointers (None: a null one)."""
+    return (ctypes.c_void_p * len(tensors))(*(0 if t is None else t.data_ptr() for t in tensors))
+
+
+def _layer_args(logits, mask):
+    """(pointers, rows, L, dtype code, mask pointer, mask rows, E) of the layers' logits, one dtype and device."""
+    require_gpu(mask, *logits)
+    E, dt = logits[0].shape[1], logits[0].dtype
+    assert all(t.dim() == 2 and t.shape[1] == E and t.dtype == dt and t.is_contiguous()
+               and t.device == logits[0].device for t in logits)
+    if mask is not None:
+        assert mask.dtype in (torch.bool, torch.uint8) and mask.dim() == 1 and mask.is_contiguous()
+        assert mask.device == logits[0].device
+    rows = (ctypes.c_int64 * len(logits))(*(t.shape[0] for t in logits))
+    return (_pointers(logits), rows, len(logits), dtype_code(dt), ptr(mask), 0 if mask is None else mask.shape[0], E)
+
+
+def aux_loss_forward(logits, top_k: int, aux_coef: float, z_coef: float, mask=None):
+    """The layers' logits, a list of (N_i, E) -> loss, load balance and z-loss (() fp32), expert_counts
+    (L, E) int32, coef (E + 1,) fp32 for ``aux_loss_backward``. mask (N,) bool or uint8: rows that count."""
+    ptrs, rows, L, code, mask_ptr, mask_rows, E = _layer_args(logits, mask)
+    dev = logits[0].device
+    losses = tuple(torch.empty((), dtype=torch.float32, device=dev) for _ in range(3))
+    counts = torch.empty(L, E, dtype=torch.int32, device=dev)
+    coef = torch.empty(E + 1, dtype=torch.float32, device=dev)
+    ws = workspace(size("pmoe_aux_loss_forward_workspace_size", rows, L, E), dev)
+    with on_device(coef):
+        call("pmoe_aux_loss_forward", ptrs, rows, L, code, mask_ptr, mask_rows, E, top_k, aux_coef, z_coef,
+             *map(ptr, losses), ptr(counts), ptr(coef), ptr(ws), ws.numel(), stream_of(coef))
+    return (*losses, counts, coef)
+
+
+def aux_loss_from_stats(counts, prob_sums, lse_sq_sums, n: int, top_k: int, aux_coef: float, z_coef: float):
+    """``aux_loss_forward`` from the routers' statistics (lists, one entry a layer) of n rows in all."""
+    require_gpu(*counts, *prob_sums, *lse_sq_sums)
+    L, E, dev = len(counts), counts[0].shape[0], counts[0].device
+    for ts, shape, dt in ((counts, (E,), torch.int32), (prob_sums, (E,), torch.float32),
+                          (lse_sq_sums, (1,), torch.float32)):
+        assert len(ts) == L and all(t.shape == shape and t.dtype == dt and t.is_contiguous() and t.device == dev
+                                    for t in ts)
+    losses = tuple(torch.empty((), dtype=torch.float32, device=dev) for _ in range(3))
+    out = torch.empty(L, E, dtype=torch.int32, device=dev)
+    coef = torch.empty(E + 1, dtype=torch.float32, device=dev)
+    ws = workspace(size("pmoe_aux_loss_from_stats_workspace_size", L, E), dev)
+    with on_device(coef):
+        call("pmoe_aux_loss_from_stats", _pointers(counts), _pointers(prob_sums), _pointers(lse_sq_sums), L, n, E,
+             top_k, aux_coef, z_coef, *map(ptr, losses), ptr(out), ptr(coef), ptr(ws), ws.numel(), stream_of(coef))
+    return (*losses, out, coef)
+
+
+def aux_loss_backward(logits, coef, grad_loss, aux_coef: float, z_coef: float, mask=None, needs=None):
+    """-> every layer's gradient (N_i, E) in its logits' dtype (None where needs[i] is false); grad_loss:
+    the loss's gradient, one fp32 value on the device."""
+    ptrs, rows, L, code, mask_ptr, mask_rows, E = _layer_args(logits, mask)
+    require_gpu(coef, grad_loss)
+    assert grad_loss.numel() == 1 and grad_loss.dtype == torch.float32 and coef.shape == (E + 1,)
+    # one allocation for all layers; each gradient is its rows
+    need = [True] * L if needs is None else [bool(x) for x in needs]
+    sizes = [t.shape[0] if k else 0 for t, k in zip(logits, need)]
+    parts = torch.empty(sum(sizes), E, dtype=logits[0].dtype, device=logits[0].device).split(sizes)
+    grads = [g if k else None for g, k in zip(parts, need)]
+    with on_device(coef):
+        call("pmoe_aux_loss_backward", ptrs, _pointers(grads), rows, L, code, mask_ptr, mask_rows, E, ptr(coef),
+             ptr(grad_loss), aux_coef, z_coef, stream_of(coef))
+    return grads
+
+
+# ------------------------------------------ activation checkpoints in 8 bits
+
+
+ACT8_GROUP = 32  # columns that share an exponent
+
+
+def act8_groups(cols: int) -> int:
+    return (cols + ACT8_GROUP - 1) // ACT8_GROUP
+
+
+def act8_save(x):
+    """x (..., C) -> codes (..., C) int8 and exps (..., ceil(C / 32)) uint8: each group of 32 columns as
+    codes in [-127, 127] times 2^(exps - 127), a value that is not finite as code -128."""
+    require_gpu(x)
+    assert x.dim() >= 1 and x.shape[-1] >= 1, "act8_save expects (..., C)"
+    x = x.contiguous()
+    C = x.shape[-1]
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    exps = torch.empty(*x.shape[:-1], act8_groups(C), dtype=torch.uint8, device=x.device)
+    with on_device(x):
+        call("pmoe_act8_save", ptr(x), dtype_code(x.dtype), codes.numel() // C, C, ptr(codes), ptr(exps),
+             stream_of(x))
+    return codes, exps
+
+
+def _check_act8(codes, exps):
+    require_gpu(codes, exps)
+    assert codes.dtype == torch.int8 and exps.dtype == torch.uint8, "an 8-bit checkpoint is int8 codes and uint8 exps"
+    assert codes.is_contiguous() and exps.is_contiguous() and codes.device == exps.device
+
+
+def act8_restore(codes, exps, dtype):
+    """The values that ``act8_save``'s codes and exps stand for, in ``dtype``."""
+    _check_act8(codes, exps)
+    C = codes.shape[-1]
+    assert exps.shape == (*codes.shape[:-1], act8_groups(C)), f"exps {tuple(exps.shape)} for codes {tuple(codes.shape)}"
+    x = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    with on_device(codes):
+        call("pmoe_act8_restore", ptr(codes), ptr(exps), codes.numel() // C, C, ptr(x), dtype_code(dtype),
+             stream_of(codes))
+    return x
+
+
+def gate_up_swiglu_act8(x, gate_up_proj, offs, row_index=None, row_weight=None):
+    """``gate_up_swiglu`` with its pre-activations kept in 8 bits: -> codes (P, 2I) int8, exps
+    (P, 2, ceil(I/32)) uint8 (gate's groups, then up's), mid (P, I), ``gate_up_swiglu``'s bit for bit."""
+    require_gpu(x, gate_up_proj, offs, row_index, row_weight)
+    E, H, I = _dims(gate_up_proj)
+    P = row_index.shape[0] if row_index is not None else x.shape[0]
+    dev, code = x.device, dtype_code(x.dtype)
+    codes = torch.empty(P, 2 * I, dtype=torch.int8, device=dev)
+    exps = torch.empty(P, 2, act8_groups(I), dtype=torch.uint8, device=dev)
+    mid = torch.empty(P, I, dtype=x.dtype, device=dev)
+    ws = workspace(size("pmoe_gate_up_swiglu_act8_workspace_size", P, E, H, I, code), dev)
+    with on_device(x):
+        call("pmoe_gate_up_swiglu_act8", ptr(x), ptr(row_index), ptr(row_weight), x.shape[0], ptr(gate_up_proj),
+             ptr(offs), code, P, E, H, I, ptr(codes), ptr(exps), ptr(mid), ptr(ws), ws.numel(), stream_of(x))
+    return codes, exps, mid
+
+
+def down_proj_dgrad_act8(grad, codes, exps, down_proj_w, offs, row_index=None, row_weight=None, need_part=False,
+                         need_mid=True):
+    """``down_proj_dgrad`` from the 8-bit checkpoint: -> grad_gate_up_out (P, 2I), mid (P, I) = row_weight *
+    silu(gate) * up of the restored values (None without need_mid), the routing-weight partials or None."""
+    _check_act8(codes, exps)
+    require_gpu(grad, down_proj_w, offs, row_index, row_weight)
+    E, H, I = down_proj_w.shape
+    P = row_index.shape[0] if row_index is not None else grad.shape[0]
+    assert codes.shape == (P, 2 * I) and exps.shape == (P, 2, act8_groups(I)), (
+        f"codes {tuple(codes.shape)}, exps {tuple(exps.shape)} for P={P}, I={I}")
+    dev, code = grad.device, dtype_code(grad.dtype)
+    ggu = torch.empty(P, 2 * I, dtype=grad.dtype, device=dev)
+    mid = torch.empty(P, I, dtype=grad.dtype, device=dev) if need_mid else None
+    part = torch.empty(P, part_cols(I), dtype=torch.float32, device=dev) if need_part else None
+    ws = workspace(size("pmoe_down_proj_dgrad_act8_workspace_size", P, E, H, I, code), dev)
+    with on_device(grad):
+        call("pmoe_down_proj_dgrad_act8", ptr(grad), ptr(row_index), ptr(row_weight), grad.shape[0], ptr(codes),
+             ptr(exps), ptr(down_proj_w), ptr(offs), code, P, E, H, I, ptr(ggu), ptr(mid), ptr(part), part_cols(I),
+             ptr(ws), ws.numel(), stream_of(grad))
+    return ggu, mid, part

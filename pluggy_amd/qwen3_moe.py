@@ -48,6 +48,9 @@ class Qwen3MoeTopKRouter(nn.Module):
 class Qwen3MoeExperts(nn.Module):
     """Packed expert weights (E, ...); dropless top-k FFN on the HIP grouped kernels."""
 
+    # set True to keep the backward's pre-activations in 8 bits (moe_expert_ffn's argument)
+    checkpoint_8bit = False
+
     def __init__(self, emb_dim: int, moe_ffn_dim: int, num_experts: int):
         super().__init__()
         self.num_experts = num_experts
@@ -58,7 +61,8 @@ class Qwen3MoeExperts(nn.Module):
 
     def forward(self, hidden_states: torch.Tensor, top_indices: torch.Tensor,
                 top_weights: torch.Tensor) -> torch.Tensor:
-        return moe_expert_ffn(hidden_states, top_indices, top_weights, self.gate_up_proj, self.down_proj)
+        return moe_expert_ffn(hidden_states, top_indices, top_weights, self.gate_up_proj, self.down_proj,
+                              checkpoint_8bit=self.checkpoint_8bit)
 
 
 class Qwen3MoeSparseMLP(nn.Module):
@@ -75,7 +79,8 @@ class Qwen3MoeSparseMLP(nn.Module):
         # router + experts as one autograd node (same arithmetic as calling
         # self.router then self.experts, which remain usable on their own)
         y, logits, stats = sparse_moe_block(flat, r.weight, self.experts.gate_up_proj, self.experts.down_proj,
-                                            r.top_k, r.norm_topk_prob, logit_bias=r.logit_bias)
+                                            r.top_k, r.norm_topk_prob, logit_bias=r.logit_bias,
+                                            checkpoint_8bit=getattr(self.experts, "checkpoint_8bit", False))
         r.last_stats = stats
         self.last_router_logits = logits
         return y.reshape(B, S, H)

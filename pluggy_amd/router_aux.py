@@ -19,6 +19,9 @@ selection instead:
   logits), for callers that only hold the logits.
 * ``router_z_loss_from_stats`` / ``expert_counts_from_stats`` - the z-loss value
   and the counts of ``_update_expert_counts`` from the same statistics.
+* ``router_aux_loss`` - both losses, the counts and every layer's gradient from
+  HIP kernels, one launch for all layers: from the logits, with rows of a padded
+  batch masked out, or from the routers' statistics.
 * ``install_stats_aux(model)`` - points a reference ``Qwen3Moe``'s
   ``_update_expert_counts`` and ``aux_loss`` at the functions above.
 """
@@ -26,11 +29,15 @@ selection instead:
 from __future__ import annotations
 
 import types
+from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
-from .moe import RouterStats
+from . import ops
+from ._lib import require_gpu
+from .moe import RouterStats, _refuse_capture, _stage
 
 
 def _totals(stats: list[RouterStats]) -> tuple[int, torch.Tensor, torch.Tensor]:
@@ -125,6 +132,97 @@ def expert_counts_from_stats(stats: list[RouterStats]) -> torch.Tensor | None:
     return torch.stack([s.expert_counts for s in stats]).sum(0).to(torch.float32).detach()
 
 
+@dataclass
+class RouterAuxLoss:
+    """What ``router_aux_loss`` returns."""
+
+    loss: torch.Tensor           # () fp32, with the logits' gradient: aux_coef * load_balance + z_coef * z_loss
+    load_balance: torch.Tensor   # () fp32, no gradient
+    z_loss: torch.Tensor         # () fp32, no gradient
+    expert_counts: torch.Tensor  # (L, E) int32: valid rows that picked each expert, by layer
+
+
+class _RouterAuxLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, top_k, aux_coef, z_coef, mask, stats, *logits):
+        with _stage("aux_loss"):
+            if stats is None:
+                *losses, counts, coef = ops.aux_loss_forward(logits, top_k, aux_coef, z_coef, mask)
+            else:
+                *losses, counts, coef = ops.aux_loss_from_stats(
+                    [s.expert_counts for s in stats], [s.prob_sum for s in stats], [s.lse_sq_sum for s in stats],
+                    sum(int(s.tokens) for s in stats), top_k, aux_coef, z_coef)
+        ctx.save_for_backward(coef, mask, *logits)
+        ctx.coefs = (aux_coef, z_coef)
+        loss, balance, z = losses
+        ctx.mark_non_differentiable(balance, z, counts)
+        ctx.set_materialize_grads(False)
+        return loss, balance, z, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_loss, _gb, _gz, _gc):
+        coef, mask, *logits = ctx.saved_tensors
+        needs = ctx.needs_input_grad[5:]
+        if g_loss is None or not any(needs):
+            return (None,) * (5 + len(logits))
+        _refuse_capture("aux_loss_bwd")
+        with _stage("aux_loss_bwd"):
+            grads = ops.aux_loss_backward(logits, coef, g_loss.float().contiguous(), *ctx.coefs, mask, needs)
+        return (None, None, None, None, None, *grads)
+
+
+@torch.compiler.disable
+def router_aux_loss(router_logits: list[torch.Tensor], num_experts: int, top_k: int,
+                    router_aux_loss_coef: float = 1.0, router_z_loss_coef: float = 0.0, *,
+                    token_mask: torch.Tensor | None = None,
+                    stats: list[RouterStats] | None = None) -> RouterAuxLoss:
+    """``Qwen3Moe.aux_loss`` and the counts of ``_update_expert_counts`` (qwen3_moe.py:417-444) on HIP.
+
+    ``loss = router_aux_loss_coef * LB + router_z_loss_coef * Z`` over the rows of
+    all layers together, as ``load_balancing_loss`` and ``router_z_loss``
+    (:285-316) define the two, with the experts selected by the fused router's
+    rule (equal logits: the lower id). ``router_logits``: one (N, E) tensor a
+    layer, all of one type (fp32, bf16 or fp16; computed in fp32). Each layer's
+    gradient has its logits' type.
+
+    ``token_mask`` (bool or integers, N entries in any shape): rows whose entry is
+    0 (the padding of a batch) count for nothing in any layer, whatever they
+    hold, and get a zero gradient; the means are over the others. No row left:
+    the losses are 0, as for no rows at all.
+
+    ``stats``: the routers' ``last_stats`` of the same layers. Value and counts
+    then come from them without a pass over the logits. They cover every row, so
+    they do not go with a mask.
+
+    Runs eagerly inside ``torch.compile`` (a graph break). A second derivative and a backward
+    under HIP graph capture are refused.
+    """
+    logits = [router_logits] if isinstance(router_logits, torch.Tensor) else list(router_logits)
+    if not logits:
+        zero = torch.tensor(0.0)
+        return RouterAuxLoss(zero, zero, zero, torch.zeros(0, num_experts, dtype=torch.int32))
+    assert 1 <= top_k <= num_experts
+    for lg in logits:
+        assert lg.dim() == 2 and lg.shape[1] == num_experts, f"router logits {tuple(lg.shape)}, expected (N, {num_experts})"
+        assert lg.dtype == logits[0].dtype and lg.device == logits[0].device, "logits of one type and device"
+    require_gpu(token_mask, *logits)
+    mask = None
+    if token_mask is not None:
+        assert stats is None, "the statistics cover every row: token_mask needs the logits alone"
+        assert not token_mask.is_floating_point() and all(lg.shape[0] == token_mask.numel() for lg in logits), (
+            f"token_mask has {token_mask.numel()} entries, the layers {[lg.shape[0] for lg in logits]} rows")
+        mask = token_mask if token_mask.dtype == torch.bool else token_mask != 0
+        mask = mask.reshape(-1).contiguous()
+    if stats is not None:
+        assert len(stats) == len(logits) and all(int(s.tokens) == lg.shape[0] for s, lg in zip(stats, logits)), (
+            "one RouterStats per layer's logits, of the same rows")
+        assert all(s.expert_counts.shape == (num_experts,) for s in stats)
+    out = _RouterAuxLoss.apply(int(top_k), float(router_aux_loss_coef), float(router_z_loss_coef), mask, stats,
+                               *(lg.contiguous() for lg in logits))
+    return RouterAuxLoss(*out)
+
+
 def _sparse_routers(model):
     from .qwen3_moe import Qwen3MoeSparseMLP
 
@@ -132,7 +230,7 @@ def _sparse_routers(model):
             if isinstance(b.ffn, Qwen3MoeSparseMLP) and b.ffn.last_router_logits is not None]
 
 
-def install_stats_aux(model) -> None:
+def install_stats_aux(model, *, fused: bool = False) -> None:
     """Make a reference ``Qwen3Moe`` (qwen3_moe.py:319-489) take its expert
     counts and load-balance loss from the kernels' routing.
 
@@ -143,6 +241,10 @@ def install_stats_aux(model) -> None:
     logits-based formula (it does not depend on the selection). The model's
     sparse blocks must be ``pluggy_amd.Qwen3MoeSparseMLP`` (installed as in the
     module-level integration), whose routers keep ``last_stats``.
+
+    With ``fused`` the loss is ``router_aux_loss``'s from those statistics: no
+    pass over the logits forward and one launch for all layers backward, in place
+    of torch operations layer by layer and a copy of all logits for the z-loss.
     """
     def _update_expert_counts(self, router_logits):
         mlps = _sparse_routers(self)
@@ -153,6 +255,10 @@ def install_stats_aux(model) -> None:
         if not logits:
             return None
         mlps = _sparse_routers(self)
+        if fused:
+            return router_aux_loss([m.last_router_logits for m in mlps], self.num_experts, mlps[0].router.top_k,
+                                   self.router_aux_loss_coef, self.router_z_loss_coef,
+                                   stats=[m.router.last_stats for m in mlps]).loss
         loss = torch.zeros((), device=logits[0].device)
         if self.router_aux_loss_coef != 0.0:
             loss = loss + self.router_aux_loss_coef * load_balancing_loss_from_stats(

@@ -1,0 +1,286 @@
+"""GPU: layer norm forward and backward against the formulas in 64 bits.
+
+Bounds, with u = 2^-24 and eps the output type's: a row's sums add at most
+64 values in a thread and a tree over 256 threads (D = 64 + 8 steps), so the mean
+is off by D u mean|x|, which counts relative to the deviation: k = (D + 16) u (1 +
+|mu| / sd) relative to the terms of each result, plus half a step (eps / 2) of
+the output type.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests._gpu_helpers import DEV, gen
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def half_step(dt):
+    return 0.0 if dt == torch.float32 else torch.finfo(dt).eps / 2
+
+
+def tiny(dt):
+    """Half of the smallest step near zero (subnormal results)."""
+    return torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2
+
+
+def reference(x, w, b, eps, g, T, H):
+    x = x.double()
+    mu = x.mean(-1, keepdim=True)
+    var = (x - mu).square().mean(-1, keepdim=True)
+    sd = (var + eps).sqrt()
+    xh = (x - mu) / sd
+    w = torch.ones(H, dtype=torch.float64, device=x.device) if w is None else w.double()
+    b = torch.zeros(H, dtype=torch.float64, device=x.device) if b is None else b.double()
+    y = xh * w + b
+    k = 88 * U * (1 + mu.abs() / sd)
+    out = {"y": (y, k * ((xh * w).abs() + w.abs() + b.abs()))}
+    if g is not None:
+        g = g.double()
+        gw = g * w
+        c1, c2 = gw.mean(-1, keepdim=True), (gw * xh).mean(-1, keepdim=True)
+        a1, a2 = gw.abs().mean(-1, keepdim=True), (gw * xh).abs().mean(-1, keepdim=True)
+        out["gx"] = ((gw - c1 - xh * c2) / sd, 2 * k * (gw.abs() + a1 + (xh.abs() + 1) * a2 + a1) / sd)
+        n = (T + 96) * U  # at most T additions, in pieces, and the joins
+        out["gw"] = ((g * xh).sum(0), n * (g * xh).abs().sum(0) + (k * g.abs()).sum(0))
+        out["gb"] = (g.sum(0), n * g.abs().sum(0))
+    return out
+
+
+def check(name, got, ref, bound):
+    dt = got.dtype
+    lim = bound + (ref.abs() + bound) * half_step(dt) + tiny(dt)
+    err = (got.double() - ref).abs()
+    worst = (err / lim).max().item() if err.numel() else 0.0
+    print(f"{name}: worst error / bound {worst:.3f}", flush=True)
+    assert worst <= 1.0, f"{name}: {worst:.3f} times the bound"
+
+
+def inputs(T, H, dt, wdt, seed, offset=0.3):
+    g = gen(seed)
+    x = (torch.randn(T, H, generator=g) * torch.exp(0.5 * torch.randn(H, generator=g)) + offset).to(DEV).to(dt)
+    w = (1 + 0.1 * torch.randn(H, generator=g)).to(DEV).to(wdt)
+    b = (0.1 * torch.randn(H, generator=g)).to(DEV).to(wdt)
+    return x, w, b, torch.randn(T, H, generator=g).to(DEV)
+
+
+SIZES = [(1, 1), (1, 2048), (3, 8), (7, 511), (5, 513), (130, 1001), (64, 1024), (65, 2040), (33, 2056), (9, 4096),
+         (7, 4104), (6, 8192), (5, 8200), (4, 16384), (3, 16385), (520, 17000), (4099, 96), (2500, 768)]
+
+
+@pytest.mark.parametrize("T,H", SIZES)
+@pytest.mark.parametrize("dt,out", [("fp32", "fp32"), ("bf16", "bf16"), ("fp16", "fp16"), ("fp32", "bf16"),
+                                    ("fp32", "fp16")])
+def test_forward_and_backward(T, H, dt, out):
+    import pluggy_amd
+
+    x, w, b, g = inputs(T, H, DT[dt], torch.float32, T * 31 + H)
+    g = g.to(DT[out])
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = pluggy_amd.layer_norm(*leaves, 1e-5, DT[out])
+    assert y.dtype == DT[out] and y.shape == x.shape
+    with torch.no_grad():
+        assert torch.equal(y, pluggy_amd.layer_norm(*leaves, 1e-5, DT[out]))
+    gx, gw, gb = torch.autograd.grad(y, leaves, g)
+    ref = reference(x, w, b, 1e-5, g, T, H)
+    for name, got in (("y", y), ("gx", gx), ("gw", gw), ("gb", gb)):
+        check(name, got.detach(), *ref[name])
+
+
+@pytest.mark.parametrize("has_w,has_b", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("wdt", ["fp32", "bf16", "fp16"])
+def test_optional_and_typed_parameters(has_w, has_b, wdt):
+    import pluggy_amd
+
+    T, H = 70, 264
+    x, w, b, g = inputs(T, H, torch.float32, DT[wdt], 5)
+    leaves = [t.requires_grad_() for t in (x, w if has_w else None, b if has_b else None) if t is not None]
+    y = pluggy_amd.layer_norm(x, w if has_w else None, b if has_b else None, 1e-6)
+    grads = dict(zip(["gx"] + ["gw"] * has_w + ["gb"] * has_b, torch.autograd.grad(y, leaves, g)))
+    ref = reference(x.detach(), w.detach() if has_w else None, b.detach() if has_b else None, 1e-6, g, T, H)
+    check("y", y.detach(), *ref["y"])
+    for name, got in grads.items():
+        check(name, got, *ref[name])
+        assert name == "gx" or got.dtype == DT[wdt]
+
+
+def test_only_the_wanted_gradients_and_mixed_parameter_types():
+    import pluggy_amd
+
+    T, H = 40, 128
+    x, w, b, g = inputs(T, H, torch.float32, torch.float32, 6)
+    b16 = b.bfloat16().requires_grad_()
+    y = pluggy_amd.layer_norm(x, w, b16)
+    (gb,) = torch.autograd.grad(y, [b16], g)
+    assert gb.dtype == torch.bfloat16
+    check("gb", gb, *reference(x, w, b16.detach(), 1e-5, g, T, H)["gb"])
+
+
+def test_large_mean_and_constant_rows():
+    """A mean far above the deviation (the variance is not a difference of large sums), and rows without any."""
+    import pluggy_amd
+
+    x, w, b, g = inputs(20, 1024, torch.float32, torch.float32, 7, offset=1000.0)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = pluggy_amd.layer_norm(*leaves)
+    ref = reference(x.detach(), w.detach(), b.detach(), 1e-5, g, 20, 1024)
+    check("y", y.detach(), *ref["y"])
+    check("gx", torch.autograd.grad(y, leaves, g)[0], *ref["gx"])
+    flat = torch.full((3, 96), 7.0, device=DEV)
+    assert torch.equal(pluggy_amd.layer_norm(flat), torch.zeros_like(flat))
+
+
+def test_not_finite_rows_stay_apart():
+    import pluggy_amd
+
+    x, w, b, g = inputs(9, 256, torch.float32, torch.float32, 8)
+    clean = pluggy_amd.layer_norm(x, w, b)
+    x[4, 17] = float("inf")
+    x[6, 0] = float("nan")
+    y = pluggy_amd.layer_norm(x, w, b)
+    for r in range(9):
+        assert y[r].isnan().all() if r in (4, 6) else torch.equal(y[r], clean[r])
+
+
+def test_shapes_strides_and_alignment():
+    import pluggy_amd
+
+    x, w, b, _ = inputs(24, 200, torch.bfloat16, torch.float32, 9)
+    y = pluggy_amd.layer_norm(x, w, b)
+    assert torch.equal(pluggy_amd.layer_norm(x.view(2, 3, 4, 200), w, b).view(24, 200), y)
+    assert torch.equal(pluggy_amd.layer_norm(x.t().contiguous().t(), w, b), y)
+    wide = torch.zeros(24, 333, dtype=torch.bfloat16, device=DEV)
+    wide[:, 1:201] = x
+    assert torch.equal(pluggy_amd.layer_norm(wide[:, 1:201], w, b), y)
+    odd = torch.zeros(24 * 200 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(24, 200)  # starts on 2 bytes
+    odd.copy_(x)
+    ref = reference(x, w, b, 1e-5, None, 24, 200)
+    check("odd", pluggy_amd.layer_norm(odd, w, b), *ref["y"])
+    assert pluggy_amd.layer_norm(x[5], w, b).shape == (200,) and torch.equal(pluggy_amd.layer_norm(x[5], w, b), y[5])
+
+
+def test_no_rows():
+    import pluggy_amd
+
+    x = torch.empty(0, 64, device=DEV, requires_grad=True)
+    w, b = (torch.ones(64, device=DEV, requires_grad=True) for _ in range(2))
+    y = pluggy_amd.layer_norm(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], torch.empty(0, 64, device=DEV))
+    assert gx.shape == (0, 64) and not gw.any() and not gb.any()
+
+
+def test_gradient_matches_differences():
+    """<grad, d> against the central difference of the 64-bit formula along d: the gradient's own error (the
+    bounds above, summed over the direction) and the difference's, h^2 times the third derivative's scale."""
+    import pluggy_amd
+
+    T, H = 6, 48
+    x, w, b, g = inputs(T, H, torch.float32, torch.float32, 10)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    grads = torch.autograd.grad(pluggy_amd.layer_norm(*leaves), leaves, g)
+    ds = [torch.randn(t.shape, generator=gen(11), dtype=torch.float64).to(DEV) for t in leaves]
+
+    def loss(h):
+        v = [t.detach().double() + h * d for t, d in zip(leaves, ds)]
+        return (reference(*v, 1e-5, None, T, H)["y"][0] * g.double()).sum()
+
+    h = 1e-4
+    want = (loss(h) - loss(-h)) / (2 * h)
+    got = sum((a.double() * d).sum() for a, d in zip(grads, ds))
+    scale = sum((a.double().abs() * d.abs()).sum() for a, d in zip(grads, ds))
+    assert abs(got - want) <= (400 * U + 100 * h * h) * scale
+
+
+def test_deterministic_and_on_another_stream():
+    import pluggy_amd
+
+    x, w, b, g = inputs(3000, 768, torch.bfloat16, torch.float32, 12)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    first = torch.autograd.grad(pluggy_amd.layer_norm(*leaves), leaves, g.bfloat16())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = torch.autograd.grad(pluggy_amd.layer_norm(*leaves), leaves, g.bfloat16())
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, c) for a, c in zip(first, second))
+
+
+def test_forward_in_a_graph_and_backward_refused_there():
+    import pluggy_amd
+
+    x, w, b, _ = inputs(50, 512, torch.bfloat16, torch.float32, 13)
+    with torch.no_grad():
+        pluggy_amd.layer_norm(x, w, b)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = pluggy_amd.layer_norm(x, w, b)
+        for k in range(3):
+            x.add_(0.5)
+            graph.replay()
+            assert torch.equal(y, pluggy_amd.layer_norm(x, w, b))
+            torch.cuda.synchronize()
+
+
+def test_backward_under_capture_raises(monkeypatch):
+    import pluggy_amd
+
+    x, w, b, g = inputs(8, 64, torch.float32, torch.float32, 14)
+    y = pluggy_amd.layer_norm(x.requires_grad_(), w, b)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="not supported under HIP graph capture"):
+        torch.autograd.grad(y, [x], g)
+
+
+def test_second_derivative_is_refused():
+    import pluggy_amd
+
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    (gx,) = torch.autograd.grad(pluggy_amd.layer_norm(x).square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()
+
+
+def test_compiled_matches_eager():
+    import pluggy_amd
+
+    x, w, b, g = inputs(33, 256, torch.float32, torch.float32, 15)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+
+    def f(x, w, b):
+        return pluggy_amd.layer_norm(x, w, b, 1e-5, torch.bfloat16) * 2
+
+    y = f(*leaves)
+    yc = torch.compile(f, backend="aot_eager", fullgraph=True)(*leaves)
+    assert torch.equal(y, yc)
+    grads = torch.autograd.grad(y, leaves, g.bfloat16()), torch.autograd.grad(yc, leaves, g.bfloat16())
+    assert all(torch.equal(a, c) for a, c in zip(*grads))
+
+
+@pytest.mark.parametrize("amp", [False, True])
+def test_moe_sublayer_with_a_layer_norm(amp):
+    """``moe_sublayer`` runs a LayerNorm block: x + mlp(layer_norm(x)) with the same calls."""
+    import pluggy_amd
+
+    B, S, H = 2, 19, 64
+    torch.manual_seed(0)
+    mlp = pluggy_amd.Qwen3MoeSparseMLP(H, 32, 8, 2).to(DEV)
+    for p in mlp.parameters():
+        torch.nn.init.normal_(p, std=0.1)
+    norm = torch.nn.LayerNorm(H).to(DEV)
+    torch.nn.init.normal_(norm.weight, mean=1.0, std=0.1)
+    x = torch.randn(B, S, H, device=DEV, requires_grad=True)
+    with torch.autocast("cuda", torch.bfloat16, enabled=amp):
+        y = pluggy_amd.moe_sublayer(x, norm, mlp)
+        normed = pluggy_amd.layer_norm(x, norm.weight, norm.bias, norm.eps, torch.bfloat16 if amp else None)
+        want = x + mlp(normed)
+    assert y.dtype == torch.float32 and torch.equal(y, want)
+    params = [x, norm.weight, norm.bias, *mlp.parameters()]
+    g = torch.randn_like(y)
+    for a, c in zip(torch.autograd.grad(y, params, g), torch.autograd.grad(want, params, g)):
+        assert torch.equal(a, c) and a.abs().sum() > 0
