@@ -56,14 +56,9 @@ __global__ __launch_bounds__(256) void act8_save_kernel(const T* __restrict__ x,
   const bool in = r < R && c < C;
   float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (in) load8<T, VEC>(x + r * C, c, C, v);
-  float a = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) a = fmaxf(a, act8_mag(v[k]));
-  a = fmaxf(a, __shfl_xor(a, 1));
-  a = fmaxf(a, __shfl_xor(a, 2));
+  uint2 w;
+  const uint32_t eb = act8_encode(v, in, w);
   if (!in) return;
-  const uint32_t eb = act8_exponent(a);
-  const uint2 w = act8_pack(v, act8_inv_scale(eb));
   int8_t* row = codes + r * C;
   if constexpr (VEC) {
     *reinterpret_cast<uint2*>(row + c) = w;
@@ -84,7 +79,7 @@ __global__ __launch_bounds__(256) void act8_restore_kernel(const int8_t* __restr
   const int c = (int)(i - r * (4 * G)) * 8;
   if (r >= R || c >= C) return;
   float v[8];
-  act8_unpack<T>(load_codes<VEC>(codes + r * C, c, C), act8_scale(exps[r * G + c / kAct8Group]), v);
+  act8_decode<T>(load_codes<VEC>(codes + r * C, c, C), exps[r * G + c / kAct8Group], v);
   store8<T, VEC>(x + r * C, c, C, v);
 }
 
@@ -103,8 +98,8 @@ __global__ __launch_bounds__(256) void act8_restore_swiglu_kernel(const int8_t* 
   const int8_t* row = codes + r * 2 * I;
   const uint8_t* er = exps + r * 2 * G + c / kAct8Group;
   float g[8], u[8], m[8];
-  act8_unpack<T>(load_codes<true>(row, c, I), act8_scale(er[0]), g);
-  act8_unpack<T>(load_codes<true>(row + I, c, I), act8_scale(er[G]), u);
+  act8_decode<T>(load_codes<true>(row, c, I), er[0], g);
+  act8_decode<T>(load_codes<true>(row + I, c, I), er[G], u);
   const float w = row_w != nullptr ? row_w[r] : 1.0f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) m[k] = g[k] * (sizeof(T) == 2 ? fast_sigmoid(g[k]) : sigmoidf_(g[k])) * u[k] * w;

@@ -1225,8 +1225,8 @@ PMOE_API int pmoe_act8_restore(const int8_t* codes, const uint8_t* exps, int64_t
 }
 
 PMOE_API size_t pmoe_gate_up_swiglu_act8_workspace_size(int64_t P, int64_t E, int64_t H, int64_t I, int dtype) {
-  (void)E; (void)H;
-  if (P <= 0 || I <= 0) return 0;
+  (void)H;
+  if (P <= 0 || I <= 0 || expert_gemm_act8(EG_GATE_UP_FWD, P, E, dtype != PMOE_F32)) return 0;
   return align_up((size_t)P * 2 * I * elem_bytes(dtype));
 }
 
@@ -1238,9 +1238,21 @@ PMOE_API int pmoe_gate_up_swiglu_act8(const void* x, const int32_t* row_index, c
   if (int rc = check_gather(row_index, x_rows, H, dtype, P, "gate_up_swiglu_act8")) return rc;
   if (P == 0) return PMOE_OK;
   PMOE_REQUIRE(x && gate_up_proj && offs && codes && exps && mid, "gate_up_swiglu_act8: null tensor");
+  PMOE_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 8 == 0, "gate_up_swiglu_act8: codes must be 8-byte aligned");
   const size_t need = pmoe_gate_up_swiglu_act8_workspace_size(P, E, H, I, dtype);
   if (workspace_bytes < need || (need > 0 && !workspace))
     return fail(PMOE_ERR_WORKSPACE, "gate_up_swiglu_act8: workspace %zu < %zu bytes", workspace_bytes, need);
+  if (expert_gemm_act8(EG_GATE_UP_FWD, P, E, dtype != PMOE_F32)) {
+    ExpertGather xg;
+    xg.index = row_index;
+    xg.rows = x_rows;
+    xg.row_w = row_weight;
+    xg.codes = codes;
+    xg.exps = exps;
+    return hip_status(dispatch_expert(EG_GATE_UP_FWD, dtype, dtype, x, gate_up_proj, nullptr, nullptr, mid, nullptr,
+                                      offs, P, E, H, I, xg, as_stream(stream)),
+                      "gate_up_swiglu_act8");
+  }
   if (int rc = pmoe_gate_up_swiglu(x, row_index, row_weight, x_rows, gate_up_proj, offs, dtype, P, E, H, I, workspace,
                                    mid, stream))
     return rc;
@@ -1248,8 +1260,8 @@ PMOE_API int pmoe_gate_up_swiglu_act8(const void* x, const int32_t* row_index, c
 }
 
 PMOE_API size_t pmoe_down_proj_dgrad_act8_workspace_size(int64_t P, int64_t E, int64_t H, int64_t I, int dtype) {
-  (void)E; (void)H;
-  if (P <= 0 || I <= 0) return 0;
+  (void)H;
+  if (P <= 0 || I <= 0 || expert_gemm_act8(EG_DOWN_DGRAD, P, E, dtype != PMOE_F32)) return 0;
   return align_up((size_t)P * 2 * I * elem_bytes(dtype)) + align_up((size_t)P * I * elem_bytes(dtype));
 }
 
@@ -1262,9 +1274,25 @@ PMOE_API int pmoe_down_proj_dgrad_act8(const void* grad, const int32_t* row_inde
   if (int rc = check_gather(row_index, grad_rows, H, dtype, P, "down_proj_dgrad_act8")) return rc;
   if (P == 0) return PMOE_OK;
   PMOE_REQUIRE(grad && codes && exps && down_proj && offs && grad_gate_up_out, "down_proj_dgrad_act8: null tensor");
+  PMOE_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 8 == 0, "down_proj_dgrad_act8: codes must be 8-byte aligned");
   const size_t need = pmoe_down_proj_dgrad_act8_workspace_size(P, E, H, I, dtype);
   if (workspace_bytes < need || (need > 0 && !workspace))
     return fail(PMOE_ERR_WORKSPACE, "down_proj_dgrad_act8: workspace %zu < %zu bytes", workspace_bytes, need);
+  if (expert_gemm_act8(EG_DOWN_DGRAD, P, E, dtype != PMOE_F32)) {
+    PMOE_REQUIRE(part == nullptr || (row_weight != nullptr && part_ld >= (I + 63) / 64),
+                 "down_proj_dgrad_act8: routing-weight partials need row_weight and part_ld >= ceil(I / 64)");
+    ExpertGather xg;
+    xg.index = row_index;
+    xg.rows = grad_rows;
+    xg.row_w = row_weight;
+    xg.part = part;
+    xg.part_ld = (int)part_ld;
+    xg.codes = const_cast<int8_t*>(codes);
+    xg.exps = const_cast<uint8_t*>(exps);
+    return hip_status(dispatch_expert(EG_DOWN_DGRAD, dtype, dtype, grad, down_proj, nullptr, grad_gate_up_out, mid,
+                                      nullptr, offs, P, E, H, I, xg, as_stream(stream)),
+                      "down_proj_dgrad_act8");
+  }
   Carver cv(workspace);
   char* gu = cv.take<char>((size_t)P * 2 * I * elem_bytes(dtype));
   char* act = mid != nullptr ? static_cast<char*>(mid) : cv.take<char>((size_t)P * I * elem_bytes(dtype));

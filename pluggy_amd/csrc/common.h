@@ -14,6 +14,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWave = 64;
 
@@ -40,6 +41,10 @@ struct ExpertGather {
   const float* row_w = nullptr;
   float* part = nullptr;
   int part_ld = 0;
+  // the 8-bit checkpoint of the pre-activations, in place of gu (act8.h):
+  // written by EG_GATE_UP_FWD, read by EG_DOWN_DGRAD
+  int8_t* codes = nullptr;
+  uint8_t* exps = nullptr;
 };
 
 

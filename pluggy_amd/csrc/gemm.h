@@ -18,6 +18,7 @@
 
 #include <type_traits>
 
+#include "act8.h"
 #include "common.h"
 
 namespace pmoe {
@@ -26,7 +27,12 @@ namespace pmoe {
 // split_chunk > 0 group g instead reduces k in [g * split_chunk, ...), a
 // split-K whose partial products land in separate C planes.
 enum GroupMode { GM_NONE = 0, GM_ROWS = 1, GM_RED = 2, GM_BATCH = 3 };
-enum EpiKind { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_SWIGLU_BWD = 2, EPI_SUM3 = 3 };
+enum EpiKind { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_SWIGLU_BWD = 2, EPI_SUM3 = 3, EPI_SWIGLU_A8 = 4, EPI_SWIGLU_BWD_A8 = 5 };
+// The SwiGLU epilogues; the A8 ones write, or read, the pre-activations as their
+// 8-bit checkpoint (act8.h) and the backward writes the activation too.
+constexpr bool epi_swiglu(int e) { return e == EPI_SWIGLU || e == EPI_SWIGLU_A8; }
+constexpr bool epi_swiglu_bwd(int e) { return e == EPI_SWIGLU_BWD || e == EPI_SWIGLU_BWD_A8; }
+constexpr bool epi_act8(int e) { return e == EPI_SWIGLU_A8 || e == EPI_SWIGLU_BWD_A8; }
 
 template <typename Tc> struct Mfma;
 
@@ -238,6 +244,9 @@ struct GemmParams {
   // accumulators times silu(g) * u (the routing weight's gradient, by block).
   const float* row_w;
   float* part; int part_ld;
+  // EPI_SWIGLU_A8: C holds the codes (P, 2 I) int8, exps (P, 2, act8_groups(I)).
+  // EPI_SWIGLU_BWD_A8: aux holds the codes; C2 / ldc2 the activation (or null).
+  uint8_t* exps;
 };
 
 struct TileInfo {
@@ -521,6 +530,7 @@ inline GemmParams zero_params() {
   p.n_index = 0;
   p.row_w = nullptr;
   p.part = nullptr; p.part_ld = 0;
+  p.exps = nullptr;
   return p;
 }
 
@@ -539,7 +549,8 @@ hipError_t launch_gemm(const GemmParams& p, hipStream_t s) {
 }
 
 // Problem description of one expert GEMM. A, B: operands as listed above;
-// aux: gu for EG_DOWN_DGRAD; C2: mid for EG_GATE_UP_FWD.
+// aux: gu for EG_DOWN_DGRAD; C2: mid for EG_GATE_UP_FWD (and for EG_DOWN_DGRAD
+// from an 8-bit checkpoint).
 template <typename T>
 GemmParams expert_params(int kind, const T* A, const T* B, const T* aux, T* C, T* C2, const int32_t* offs, int P,
                          int E, int H, int I, const ExpertGather& xg = ExpertGather()) {
@@ -598,6 +609,11 @@ GemmParams expert_params(int kind, const T* A, const T* B, const T* aux, T* C, T
   }
   if (kind == EG_GATE_UP_FWD || kind == EG_DOWN_DGRAD) p.row_w = xg.row_w;
   if (kind == EG_DOWN_DGRAD) { p.part = xg.part; p.part_ld = xg.part_ld; }
+  if (xg.exps != nullptr) {
+    p.exps = xg.exps;
+    if (kind == EG_GATE_UP_FWD) p.C = xg.codes;
+    if (kind == EG_DOWN_DGRAD) { p.aux = xg.codes; p.C2 = C2; p.ldc2 = I; }
+  }
   return p;
 }
 

@@ -137,6 +137,11 @@ int expert_gemm_tile_rows(int kind, int P, int E, int H, int I, bool half, int c
   return DmaExpert::BM;
 }
 
+bool expert_gemm_act8(int kind, int64_t P, int64_t E, bool half) {
+  if (!half) return false;
+  return kind == EG_DOWN_DGRAD || (kind == EG_GATE_UP_FWD && P > (int64_t)kDecodeRowsPerExpert * E);
+}
+
 template <typename T, typename Tw>
 hipError_t expert_gemm_run(int kind, const T* A, const T* B, const T* aux, T* C, T* C2, Tw* Cw, const int32_t* offs,
                            int P, int E, int H, int I, const ExpertGather& xg, hipStream_t s) {

@@ -173,7 +173,11 @@ __device__ __forceinline__ void store_tile_full_cols(const f32x16 (&acc)[Cfg::MI
 // MI355X at config 2: 0.300 ms against 0.321 ms for the slab loop in
 // store_slabs, with PF = 1, 2 and 3 alike. The arithmetic and its order are
 // those of that slab loop.
-template <class Cfg, bool NT>
+//
+// A8: the pre-activations come as int8 codes and a power of two per 32 columns
+// (four lanes), half the bytes to read, and the activation w silu(g) u goes out
+// as well: the weight gradient's operand, which the forward then need not keep.
+template <class Cfg, bool NT, bool A8>
 __device__ __forceinline__ void store_tile_swiglu_bwd(const f32x16 (&acc)[Cfg::MI][Cfg::NI], float* stage,
                                                       const TileInfo& ti, const GemmParams& p, int wm, int wn,
                                                       int lane, int blocks) {
@@ -187,10 +191,18 @@ __device__ __forceinline__ void store_tile_swiglu_bwd(const f32x16 (&acc)[Cfg::M
   const int col0 = __builtin_amdgcn_readfirstlane(ti.n0 + wn * WN);
   const int r = lane / CPR, c = (lane % CPR) * 8;
   const int ldaux = (int)p.ldaux, ldc = (int)p.ldc;
-  const T16* GU = reinterpret_cast<const T16*>(p.aux) + (int64_t)row0 * p.ldaux;
+  constexpr int AB = A8 ? 1 : 2;  // bytes of a saved pre-activation
+  const char* GU = reinterpret_cast<const char*>(p.aux) + (int64_t)row0 * p.ldaux * AB;
   T16* DG = reinterpret_cast<T16*>(p.C) + (int64_t)row0 * p.ldc;
   const __amdgpu_buffer_rsrc_t rs_gu =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<T16*>(GU), (short)0, rows * ldaux * 2, 0x00020000);
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(GU), (short)0, rows * ldaux * AB, 0x00020000);
+  const int lde = A8 ? 2 * act8_groups(p.inter) : 0;  // exponent bytes of a row
+  const bool has_mid = A8 && p.C2 != nullptr;
+  const __amdgpu_buffer_rsrc_t rs_ex = __builtin_amdgcn_make_buffer_rsrc(
+      A8 ? p.exps + (int64_t)row0 * lde : nullptr, (short)0, A8 ? rows * lde : 0, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rs_mid = __builtin_amdgcn_make_buffer_rsrc(
+      has_mid ? reinterpret_cast<T16*>(p.C2) + (int64_t)row0 * p.ldc2 : nullptr, (short)0,
+      has_mid ? rows * (int)p.ldc2 * 2 : 0, 0x00020000);
   const __amdgpu_buffer_rsrc_t rs_dg = __builtin_amdgcn_make_buffer_rsrc(DG, (short)0, rows * ldc * 2, 0x00020000);
   const bool has_w = p.row_w != nullptr, has_part = p.part != nullptr;
   const __amdgpu_buffer_rsrc_t rs_w = __builtin_amdgcn_make_buffer_rsrc(
@@ -200,18 +212,29 @@ __device__ __forceinline__ void store_tile_swiglu_bwd(const f32x16 (&acc)[Cfg::M
       0x00020000);
   constexpr int AUX = NT ? 2 : 0;
   const int half = lane >> 5, col_l = lane & 31;
-  u32x4 pg[PF], pu[PF];
+  u32x4 pg[PF], pu[PF];  // A8: the codes in the first two words, the exponent byte in the third
   float pw[PF];
   // slab s: rows 8 (s % 4) .. +7 of the wave's block s / 4; this lane's row in it is r
   // per-lane offsets are fixed; the slab's first row and the column block go
   // in the uniform (SGPR) offset, so the unrolled slabs share four VGPRs
-  const int vo_gu = (r * ldaux + c) * 2, vo_dg = (r * ldc + c) * 2, vo_w = r * 4, vo_part = r * p.part_ld * 4;
+  const int vo_gu = (r * ldaux + c) * AB, vo_dg = (r * ldc + c) * 2, vo_w = r * 4, vo_part = r * p.part_ld * 4;
+  const int vo_ex = r * lde + c / kAct8Group, vo_mid = A8 ? (r * (int)p.ldc2 + c) * 2 : 0;
   auto fetch = [&](auto sc) {
     constexpr int S = decltype(sc)::value;
     constexpr int R0 = Cfg::row_blk(S / 4) + 8 * (S % 4);
-    const int so = (R0 * ldaux + col0) * 2;
-    pg[S % PF] = __builtin_amdgcn_raw_buffer_load_b128(rs_gu, vo_gu, so, 0);
-    pu[S % PF] = __builtin_amdgcn_raw_buffer_load_b128(rs_gu, vo_gu, so + (int)p.inter * 2, 0);
+    const int so = (R0 * ldaux + col0) * AB;
+    if constexpr (A8) {
+      const u32x2 wg = __builtin_amdgcn_raw_buffer_load_b64(rs_gu, vo_gu, so, 0);
+      const u32x2 wu = __builtin_amdgcn_raw_buffer_load_b64(rs_gu, vo_gu, so + (int)p.inter, 0);
+      const int se = R0 * lde + col0 / kAct8Group;
+      const uint32_t eg = __builtin_amdgcn_raw_buffer_load_b8(rs_ex, vo_ex, se, 0);
+      const uint32_t eu = __builtin_amdgcn_raw_buffer_load_b8(rs_ex, vo_ex, se + lde / 2, 0);
+      pg[S % PF] = u32x4{wg[0], wg[1], eg, 0u};
+      pu[S % PF] = u32x4{wu[0], wu[1], eu, 0u};
+    } else {
+      pg[S % PF] = __builtin_amdgcn_raw_buffer_load_b128(rs_gu, vo_gu, so, 0);
+      pu[S % PF] = __builtin_amdgcn_raw_buffer_load_b128(rs_gu, vo_gu, so + (int)p.inter * 2, 0);
+    }
     pw[S % PF] = has_w ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs_w, vo_w, R0 * 4, 0)) : 1.0f;
   };
   static_for<0, PF>([&](auto sc) { fetch(sc); });
@@ -222,10 +245,15 @@ __device__ __forceinline__ void store_tile_swiglu_bwd(const f32x16 (&acc)[Cfg::M
     for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int rr = 0; rr < 4; ++rr) stage_put(stage, 4 * half + rr, j * 32 + col_l, acc[i][j][4 * q + rr]);
-    float v[8], g[8], u[8], dg[8], du[8];
+    float v[8], g[8], u[8], dg[8], du[8], m[8];
     stage_get8(stage, r, c, v);
-    unpack8<T16>(pg[S % PF], g);
-    unpack8<T16>(pu[S % PF], u);
+    if constexpr (A8) {
+      act8_decode<T16>(make_uint2(pg[S % PF][0], pg[S % PF][1]), pg[S % PF][2], g);
+      act8_decode<T16>(make_uint2(pu[S % PF][0], pu[S % PF][1]), pu[S % PF][2], u);
+    } else {
+      unpack8<T16>(pg[S % PF], g);
+      unpack8<T16>(pu[S % PF], u);
+    }
     const float ws = pw[S % PF];
     if constexpr (S + PF < NSLAB) fetch(std::integral_constant<int, S + PF>());
     float pd = 0.0f;
@@ -234,11 +262,15 @@ __device__ __forceinline__ void store_tile_swiglu_bwd(const f32x16 (&acc)[Cfg::M
       const float sg = fast_sigmoid(g[t]);
       const float silu = g[t] * sg;
       pd += v[t] * (silu * u[t]);
+      if constexpr (A8) m[t] = silu * u[t] * ws;
       const float dm = v[t] * ws;
       dg[t] = dm * u[t] * (sg + silu * (1.0f - sg));
       du[t] = dm * silu;
     }
     constexpr int R0 = Cfg::row_blk(i) + 8 * q;
+    if constexpr (A8)
+      if (has_mid)
+        __builtin_amdgcn_raw_buffer_store_b128(Out8<T16>::pack(m), rs_mid, vo_mid, (R0 * (int)p.ldc2 + col0) * 2, AUX);
     const int so = (R0 * ldc + col0) * 2;
     __builtin_amdgcn_raw_buffer_store_b128(Out8<T16>::pack(dg), rs_dg, vo_dg, so, AUX);
     __builtin_amdgcn_raw_buffer_store_b128(Out8<T16>::pack(du), rs_dg, vo_dg, so + (int)p.inter * 2, AUX);
@@ -263,13 +295,14 @@ __device__ __forceinline__ void store_slabs(const f32x16 (&acc)[Cfg::MI][Cfg::NI
   constexpr int LD = PersistLayout<Cfg>::EPI_LD;
   constexpr int LDW = EpiStage<Cfg, PACK, SLAB>::ROW;  // packed: words per staged row
   constexpr int QPS = SLAB / 8, NSL = 32 / SLAB;         // row groups q per slab, slabs per 32-row block
-  static_assert(!PACK || (sizeof(Tout) == 2 && EPI != EPI_SWIGLU_BWD), "packed staging of bf16 outputs");
+  static_assert(!PACK || (sizeof(Tout) == 2 && !epi_swiglu_bwd(EPI)), "packed staging of bf16 outputs");
+  static_assert(EPI != EPI_SWIGLU_A8 || WN == 64, "a wave tile's 32 gate columns are one group of the checkpoint");
   static_assert(EPI == EPI_STORE || sizeof(Tout) == 2, "fused epilogues write bf16");
   constexpr bool NT = nt_epilogue<GM>();
-  if constexpr (EPI == EPI_SWIGLU_BWD && GM == GM_ROWS && Cfg::WN == 64) {
+  if constexpr (epi_swiglu_bwd(EPI) && GM == GM_ROWS && Cfg::WN == 64) {
     if (ti.n0 + Cfg::BN <= p.N && (int64_t)Cfg::ROW_SPAN * p.ldaux * 2 < ((int64_t)1 << 31) &&
         (int64_t)Cfg::ROW_SPAN * p.ldc * 2 < ((int64_t)1 << 31)) {
-      store_tile_swiglu_bwd<Cfg, NT>(acc, stage, ti, p, wm, wn, lane, blocks);
+      store_tile_swiglu_bwd<Cfg, NT, epi_act8(EPI)>(acc, stage, ti, p, wm, wn, lane, blocks);
       return;
     }
   }
@@ -287,7 +320,7 @@ __device__ __forceinline__ void store_slabs(const f32x16 (&acc)[Cfg::MI][Cfg::NI
   // before the first slab rather than one global load (and its latency) per slab
   constexpr int SW_CPR = WN / 2 / 8, SW_NE = (SLAB * SW_CPR + 63) / 64;
   float wsp[MI][NSL][SW_NE];
-  if constexpr (EPI == EPI_SWIGLU) {
+  if constexpr (epi_swiglu(EPI)) {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -331,7 +364,35 @@ __device__ __forceinline__ void store_slabs(const f32x16 (&acc)[Cfg::MI][Cfg::NI
       __builtin_amdgcn_s_waitcnt((15) | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0): slab written
       asm volatile("" ::: "memory");
       const int row_base = ti.m0 + Cfg::wave_row(wm) + Cfg::row_blk(i) + SLAB * hs;
-      if constexpr (EPI == EPI_SWIGLU) {
+      if constexpr (EPI == EPI_SWIGLU_A8) {
+        // four lanes a row: a group of the checkpoint each of gate and up
+        constexpr int CPR = 4;
+        static_assert(SLAB * CPR == kWave && WN / 2 == kAct8Group, "one chunk per lane per slab");
+        const int r = lane / CPR, c = (lane % CPR) * 8;
+        const int row = row_base + r, col = ti.n0 + wn * (WN / 2) + c;
+        const u32x4 gw = *reinterpret_cast<const u32x4*>(st32 + r * LDW + c / 2);  // rounded: the saved values
+        const u32x4 uw = *reinterpret_cast<const u32x4*>(st32 + r * LDW + WN / 4 + c / 2);
+        uint2 qg, qu;
+        const uint32_t eg = act8_encode16<Tout>(gw, col < p.inter, qg), eu = act8_encode16<Tout>(uw, col < p.inter, qu);
+        if (row < ti.m_end && col < p.inter) {
+          int8_t* codes = reinterpret_cast<int8_t*>(p.C) + (int64_t)row * p.ldc + col;
+          *reinterpret_cast<uint2*>(codes) = qg;
+          *reinterpret_cast<uint2*>(codes + p.inter) = qu;
+          if (lane % CPR == 0) {
+            const int G = act8_groups(p.inter);
+            uint8_t* ex = p.exps + (int64_t)row * 2 * G + col / kAct8Group;
+            ex[0] = (uint8_t)eg;
+            ex[G] = (uint8_t)eu;
+          }
+          const float ws = wsp[i][hs][0];
+          float g[8], u[8], m[8];
+          unpack8<Tout>(gw, g);
+          unpack8<Tout>(uw, u);
+#pragma unroll
+          for (int t = 0; t < 8; ++t) m[t] = g[t] * fast_sigmoid(g[t]) * u[t] * ws;
+          st_out8<NT>(reinterpret_cast<Tout*>(p.C2) + (int64_t)row * p.ldc2 + col, m);
+        }
+      } else if constexpr (EPI == EPI_SWIGLU) {
         constexpr int H2 = WN / 2, CPR = H2 / 8;
         Tout* MID = reinterpret_cast<Tout*>(p.C2);
 #pragma unroll
@@ -357,7 +418,7 @@ __device__ __forceinline__ void store_slabs(const f32x16 (&acc)[Cfg::MI][Cfg::NI
         }
       } else {
         constexpr int CPR = WN / 8;
-        static_assert(EPI != EPI_SWIGLU_BWD || WN == 64, "routing-weight partials are per 64-column block");
+        static_assert(!epi_swiglu_bwd(EPI) || WN == 64, "routing-weight partials are per 64-column block");
         const int col_base = ti.n0 + wn * WN;
 #pragma unroll
         for (int ei = 0; ei < (SLAB * CPR + 63) / 64; ++ei) {
@@ -376,23 +437,34 @@ __device__ __forceinline__ void store_slabs(const f32x16 (&acc)[Cfg::MI][Cfg::NI
                 unpack8<Tout>(w, v);
                 for (int t = 0; col + t < p.N; ++t) store_scalar<Tout>(C + (int64_t)row * p.ldc + col + t, v[t]);
               }
-            } else if constexpr (EPI == EPI_SWIGLU_BWD) {
+            } else if constexpr (epi_swiglu_bwd(EPI)) {
               // v = d(mid), or with row_w d(w * mid): then d(mid) = w v and d(w) += v . mid
               Vec8<float>::load(stage + r * LD + c, v);
-              const Tout* GU = reinterpret_cast<const Tout*>(p.aux) + (int64_t)row * p.ldaux;
-              float g[8], u[8], dg[8], du[8];
-              Vec8<Tout>::load(GU + col, g);
-              Vec8<Tout>::load(GU + p.inter + col, u);
+              float g[8], u[8], dg[8], du[8], m[8];
+              if constexpr (epi_act8(EPI)) {
+                const int8_t* codes = reinterpret_cast<const int8_t*>(p.aux) + (int64_t)row * p.ldaux + col;
+                const int G = act8_groups(p.inter);
+                const uint8_t* ex = p.exps + (int64_t)row * 2 * G + col / kAct8Group;
+                act8_decode<Tout>(*reinterpret_cast<const uint2*>(codes), ex[0], g);
+                act8_decode<Tout>(*reinterpret_cast<const uint2*>(codes + p.inter), ex[G], u);
+              } else {
+                const Tout* GU = reinterpret_cast<const Tout*>(p.aux) + (int64_t)row * p.ldaux;
+                Vec8<Tout>::load(GU + col, g);
+                Vec8<Tout>::load(GU + p.inter + col, u);
+              }
               const float ws = p.row_w != nullptr ? p.row_w[row] : 1.0f;
 #pragma unroll
               for (int t = 0; t < 8; ++t) {
                 const float sg = fast_sigmoid(g[t]);
                 const float silu = g[t] * sg;
                 pd += v[t] * (silu * u[t]);
+                if constexpr (epi_act8(EPI)) m[t] = silu * u[t] * ws;
                 const float dm = v[t] * ws;
                 dg[t] = dm * u[t] * (sg + silu * (1.0f - sg));
                 du[t] = dm * silu;
               }
+              if constexpr (epi_act8(EPI))
+                if (p.C2 != nullptr) st_out8<NT>(reinterpret_cast<Tout*>(p.C2) + (int64_t)row * p.ldc2 + col, m);
               st_out8<NT>(C + (int64_t)row * p.ldc + col, dg);
               st_out8<NT>(C + (int64_t)row * p.ldc + p.inter + col, du);
             } else {
@@ -404,7 +476,7 @@ __device__ __forceinline__ void store_slabs(const f32x16 (&acc)[Cfg::MI][Cfg::NI
               }
             }
           }
-          if constexpr (EPI == EPI_SWIGLU_BWD) {
+          if constexpr (epi_swiglu_bwd(EPI)) {
             if (p.part != nullptr) {  // the CPR = 8 lanes of a row are consecutive: sum them in a fixed order
               pd += __shfl_xor(pd, 1);
               pd += __shfl_xor(pd, 2);
@@ -717,15 +789,15 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_persist_kernel(GemmPa
   constexpr int MI = Cfg::MI, NI = Cfg::NI;
   constexpr int SLOT = Cfg::STAGE_BYTES;  // ring slot bytes
   // bf16 outputs stage packed (the SwiGLU backward reads its fp32 accumulators back)
-  constexpr bool PACK = sizeof(Tout) == 2 && (EPI == EPI_SWIGLU || EPI == EPI_STORE);
-  static_assert(PACK || EPI != EPI_SWIGLU, "the SwiGLU forward stages packed bf16");
+  constexpr bool PACK = sizeof(Tout) == 2 && (epi_swiglu(EPI) || EPI == EPI_STORE);
+  static_assert(PACK || !epi_swiglu(EPI), "the SwiGLU forward stages packed bf16");
   // (a plain store may round to the other 16-bit format: the router's input
   // gradient from bf16 pieces of an fp16 weight)
   static_assert(sizeof(Tout) == 4 || std::is_same<Tout, typename Cfg::Tc>::value || EPI == EPI_STORE,
                 "16-bit outputs of the fused epilogues are in the operands' format");
   static_assert(GM == GM_ROWS || GM == GM_RED, "persistent kernel serves the expert GEMMs");
   static_assert(!(GM == GM_RED && (A_KC || B_KC)), "GM_RED expects [k][m] and [k][n] operands");
-  static_assert(EPI != EPI_SWIGLU || (B_KC && GM == GM_ROWS && Cfg::WN % 32 == 0), "SwiGLU epilogue layout");
+  static_assert(!epi_swiglu(EPI) || (B_KC && GM == GM_ROWS && Cfg::WN % 32 == 0), "SwiGLU epilogue layout");
   static_assert(GATH == G_NONE || (GATH == GA_ROWS && GM == GM_ROWS && A_KC) ||
                     ((GATH == GA_KROWS || GATH == GB_KROWS) && GM == GM_RED),
                 "gathers: A's rows in GM_ROWS, A's or B's k-rows in GM_RED");
@@ -746,7 +818,7 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_persist_kernel(GemmPa
   const int groups = p.groups;
 
   TileWalk<Cfg, GM> walk;
-  if (!walk.init(p, (EPI == EPI_SWIGLU) ? p.inter : p.N, (EPI == EPI_SWIGLU) ? BN / 2 : BN, s_offs, s_scan, s_order,
+  if (!walk.init(p, epi_swiglu(EPI) ? p.inter : p.N, epi_swiglu(EPI) ? BN / 2 : BN, s_offs, s_scan, s_order,
                  &s_cmax, s_deal, smem))
     return;
   const int ntiles_n = walk.ntiles_n, mt_red = walk.mt_red, mb = walk.mb;
@@ -777,7 +849,7 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_persist_kernel(GemmPa
   // NS - 1 >= 2 stages were fetched before it started; with two slots stage 1
   // would be issued during stage 0 and read before it had landed.
   static_assert(NS >= 3, "the persistent ring needs three slots or more");
-  constexpr int SPREAD = ((EPI == EPI_SWIGLU && KS == 2) || (NS == 4 && GM == GM_ROWS)) ? KS : KS - 1;
+  constexpr int SPREAD = ((epi_swiglu(EPI) && KS == 2) || (NS == 4 && GM == GM_ROWS)) ? KS : KS - 1;
   constexpr int TOTM = SPREAD * MI * NI;  // MFMA slots the DMAs are spread over (several may share one)
   static_assert(SPREAD >= 1, "the DMAs of a stage need MFMA slots");
   // The stage's DMAs issued before its barrier. At that barrier stream stage
@@ -836,7 +908,7 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_persist_kernel(GemmPa
         T.ti.k_lo = g == 0 ? 0 : s_offs[g - 1];
         T.ti.k_hi = s_offs[g];
       }
-      T.ti.n0 = (EPI == EPI_SWIGLU) ? tn * (BN / 2) : tn * BN;
+      T.ti.n0 = epi_swiglu(EPI) ? tn * (BN / 2) : tn * BN;
       if constexpr (A_KC) {
         if constexpr (GATH == GA_ROWS) {
           a_bytes = p.a_bytes;  // the whole gathered storage
@@ -870,7 +942,7 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_persist_kernel(GemmPa
     // WN/2 gate columns then the matching up columns
     const int n0 = T.ti.n0, N = p.N, I = p.inter;
     auto b_row_of = [&](int c) {
-      if constexpr (EPI == EPI_SWIGLU) {
+      if constexpr (epi_swiglu(EPI)) {
         const int w = c / Cfg::WN, cc = c % Cfg::WN, h = Cfg::WN / 2;
         const int gcol = n0 + w * h + (cc % h);
         if (gcol >= I) return -1;
@@ -1154,10 +1226,18 @@ hipError_t expert_gemm_persist_rows(int kind, const T16* A, const T16* B, const 
   const bool gath = xg.index != nullptr;
   switch (kind) {
     case EG_GATE_UP_FWD:
+      if (p.exps != nullptr) {
+        if (gath) return launch_gemm_persist<Cfg, true, true, GM_ROWS, EPI_SWIGLU_A8, T16, GA_ROWS>(p, num_cus, s);
+        return launch_gemm_persist<Cfg, true, true, GM_ROWS, EPI_SWIGLU_A8>(p, num_cus, s);
+      }
       if (gath) return launch_gemm_persist<Cfg, true, true, GM_ROWS, EPI_SWIGLU, T16, GA_ROWS>(p, num_cus, s);
       return launch_gemm_persist<Cfg, true, true, GM_ROWS, EPI_SWIGLU>(p, num_cus, s);
     case EG_DOWN_FWD: return launch_gemm_persist<Cfg, true, true, GM_ROWS, EPI_STORE>(p, num_cus, s);
     case EG_DOWN_DGRAD:
+      if (p.exps != nullptr) {
+        if (gath) return launch_gemm_persist<Cfg, true, false, GM_ROWS, EPI_SWIGLU_BWD_A8, T16, GA_ROWS>(p, num_cus, s);
+        return launch_gemm_persist<Cfg, true, false, GM_ROWS, EPI_SWIGLU_BWD_A8>(p, num_cus, s);
+      }
       if (gath) return launch_gemm_persist<Cfg, true, false, GM_ROWS, EPI_SWIGLU_BWD, T16, GA_ROWS>(p, num_cus, s);
       return launch_gemm_persist<Cfg, true, false, GM_ROWS, EPI_SWIGLU_BWD>(p, num_cus, s);
     case EG_GATE_UP_DGRAD: return launch_gemm_persist<Cfg, true, false, GM_ROWS, EPI_STORE>(p, num_cus, s);

@@ -57,11 +57,11 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_pp_kernel(GemmParams 
   constexpr int BM = Cfg::BM, BN = Cfg::BN, BK = Cfg::BK, NW = Cfg::NW, UNIT = Cfg::UNIT;
   constexpr int MI = Cfg::MI, NI = Cfg::NI;
   static_assert(BM == 256 && BN == 256 && BK == 64 && NW == 8 && MI == 4 && NI == 2, "ping-pong tile shape");
-  constexpr bool PACK = sizeof(Tout) == 2 && (EPI == EPI_SWIGLU || EPI == EPI_STORE);
-  static_assert(PACK || EPI != EPI_SWIGLU, "the SwiGLU forward stages packed bf16");
+  constexpr bool PACK = sizeof(Tout) == 2 && (epi_swiglu(EPI) || EPI == EPI_STORE);
+  static_assert(PACK || !epi_swiglu(EPI), "the SwiGLU forward stages packed bf16");
   static_assert(sizeof(Tout) == 4 || std::is_same<Tout, typename Cfg::Tc>::value || EPI == EPI_STORE,
                 "16-bit outputs of the fused epilogues are in the operands' format");
-  static_assert(EPI != EPI_SWIGLU || B_KC, "SwiGLU epilogue layout");
+  static_assert(!epi_swiglu(EPI) || B_KC, "SwiGLU epilogue layout");
   static_assert(GATH == G_NONE || GATH == GA_ROWS, "gathers: A's rows");
 
   // [A: parity 0 (A0, A1), parity 1][N: parity 0 (N0, N1), parity 1]
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_pp_kernel(GemmParams 
   const int groups = p.groups;
 
   TileWalk<Cfg, GM_ROWS> walk;
-  if (!walk.init(p, (EPI == EPI_SWIGLU) ? p.inter : p.N, (EPI == EPI_SWIGLU) ? BN / 2 : BN, s_offs, s_scan, nullptr,
+  if (!walk.init(p, epi_swiglu(EPI) ? p.inter : p.N, epi_swiglu(EPI) ? BN / 2 : BN, s_offs, s_scan, nullptr,
                  nullptr, nullptr, nullptr))
     return;
 
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_pp_kernel(GemmParams 
         e[0] = g;
         e[1] = (g == 0 ? 0 : s_offs[g - 1]) + mt * BM;
         e[2] = s_offs[g];
-        e[3] = tn * (EPI == EPI_SWIGLU ? BN / 2 : BN);
+        e[3] = tn * (epi_swiglu(EPI) ? BN / 2 : BN);
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) s_tile[(first + tid) & 63][x] = e[x];
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_pp_kernel(GemmParams 
     // Byte offsets of this lane's chunks (kOOB: none). The four of an operand's
     // k tile (two units of two instructions) lie at fixed distances, except
     // for gathered rows and SwiGLU columns (which end inside B, not at its end).
-    uint32_t a[GATH == GA_ROWS ? 4 : 1], b[EPI == EPI_SWIGLU ? 2 : 1];
+    uint32_t a[GATH == GA_ROWS ? 4 : 1], b[epi_swiglu(EPI) ? 2 : 1];
     bool half;  // at most 128 rows: A1 is neither fetched nor read
     // a half tile that is its group's only m-tile: no other tile reads its B, which
     // streams in with non-temporal loads (1200 tokens of the Qwen3-30B-A3B layer:
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_pp_kernel(GemmParams 
     } else {
       T.a[0] = (uint32_t)r0 * lda2 + (uint32_t)(kc_k * 2);
     }
-    if constexpr (EPI == EPI_SWIGLU) {
+    if constexpr (epi_swiglu(EPI)) {
       // N halves: half 0 holds gate columns (LDS row r: tile column r), half 1 the matching up columns
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(Cfg::NT, 1) void grouped_gemm_pp_kernel(GemmParams 
         const uint32_t k2 = (uint32_t)(k0 * 2);
         if constexpr (IS_A && GATH == GA_ROWS) v[i] = T.a[2 * HALF + i] + k2;
         else if constexpr (IS_A) v[i] = T.a[0] + (k2 + (uint32_t)(128 * HALF + 64 * i) * lda2);
-        else if constexpr (EPI == EPI_SWIGLU) v[i] = T.b[i] + (k2 + (HALF ? (uint32_t)p.inter * ldb2 : 0u));
+        else if constexpr (epi_swiglu(EPI)) v[i] = T.b[i] + (k2 + (HALF ? (uint32_t)p.inter * ldb2 : 0u));
         else v[i] = T.b[0] + (k2 + (uint32_t)(32 * HALF + 128 * i) * ldb2);
         if constexpr (!WHOLE) v[i] = k0 + BK > p.K && k0 + kc_k >= p.K ? kOOB : v[i];  // the k tail
       }
@@ -458,10 +458,18 @@ hipError_t expert_gemm_pp_rows(int kind, const T16* A, const T16* B, const T16* 
   const bool gath = xg.index != nullptr;
   switch (kind) {
     case EG_GATE_UP_FWD:
+      if (p.exps != nullptr) {
+        if (gath) return launch_gemm_pp<Cfg, true, EPI_SWIGLU_A8, GA_ROWS>(p, num_cus, s);
+        return launch_gemm_pp<Cfg, true, EPI_SWIGLU_A8>(p, num_cus, s);
+      }
       if (gath) return launch_gemm_pp<Cfg, true, EPI_SWIGLU, GA_ROWS>(p, num_cus, s);
       return launch_gemm_pp<Cfg, true, EPI_SWIGLU>(p, num_cus, s);
     case EG_DOWN_FWD: return launch_gemm_pp<Cfg, true, EPI_STORE>(p, num_cus, s);
     case EG_DOWN_DGRAD:
+      if (p.exps != nullptr) {
+        if (gath) return launch_gemm_pp<Cfg, false, EPI_SWIGLU_BWD_A8, GA_ROWS>(p, num_cus, s);
+        return launch_gemm_pp<Cfg, false, EPI_SWIGLU_BWD_A8>(p, num_cus, s);
+      }
       if (gath) return launch_gemm_pp<Cfg, false, EPI_SWIGLU_BWD, GA_ROWS>(p, num_cus, s);
       return launch_gemm_pp<Cfg, false, EPI_SWIGLU_BWD>(p, num_cus, s);
     case EG_GATE_UP_DGRAD: return launch_gemm_pp<Cfg, false, EPI_STORE>(p, num_cus, s);

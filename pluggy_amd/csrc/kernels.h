@@ -26,6 +26,12 @@ hipError_t expert_gemm_run(int kind, const T* A, const T* B, const T* aux, T* C,
 // compute units (<= 0: the current device's).
 int expert_gemm_tile_rows(int kind, int P, int E, int H, int I, bool half, int cus);
 
+// Whether expert GEMM `kind` (gate_up forward, down dgrad) writes, or reads, the
+// 8-bit checkpoint in its own epilogue (ExpertGather::codes): the 16-bit engines
+// do, except the forward's tiles for few-token batches, whose waves hold half a
+// group of 32 columns; the fp32 engine does not.
+bool expert_gemm_act8(int kind, int64_t P, int64_t E, bool half);
+
 // ---- router GEMMs in fp32 arithmetic (gemm.hip). TX: x dtype, TW: router weight dtype.
 template <typename TX, typename TW>
 hipError_t router_logits_gemm(const TX* x, const TW* w, int T, int H, int E, float* logits, hipStream_t s);
