@@ -35,8 +35,8 @@ __device__ __forceinline__ float act8_inv_scale(uint32_t eb) { return __uint_as_
 
 // The largest of four lanes' values (a group), in each of them (DPP quad permutations).
 __device__ __forceinline__ uint32_t act8_quad_max(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));
-  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));
 }
 
 constexpr uint32_t kAct8Inf = 0x7f800000u;

@@ -971,7 +971,7 @@ int check_aux(const void* const* arrays, const int64_t* rows, int64_t L, int64_t
     total += rows[i];
   }
   PMOE_REQUIRE(total <= kMaxIndex, "%s: %lld rows in all", what, (long long)total);
-  plan->bpl = aux_blocks_per_layer((int)L, plan->rows);
+  plan->bpl = aux_blocks_per_layer((int)L, plan->rows, (int)E);
   return PMOE_OK;
 }
 
@@ -985,7 +985,7 @@ int check_mask(const uint8_t* mask, int64_t mask_rows, const int64_t* rows, int6
 
 size_t aux_bytes(int64_t L, int bpl, int64_t E) {
   const size_t nb = (size_t)L * bpl;
-  return 2 * align_up(nb * E * 4) + 2 * align_up(nb * 4) + 2 * align_up((size_t)E * 8);
+  return 2 * align_up(nb * E * 4) + 2 * align_up(nb * 4) + 2 * align_up((size_t)E * 8) + align_up(4);
 }
 
 AuxLayers layer_table(const void* const* logits, const int64_t* rows, int64_t first, int n) {
@@ -1001,7 +1001,7 @@ PMOE_API size_t pmoe_aux_loss_forward_workspace_size(const int64_t* row_counts, 
   if (row_counts == nullptr || L < 1 || L > 4096 || E < 1 || E > 1024) return 0;
   int64_t most = 0;
   for (int64_t i = 0; i < L; ++i) most = std::max(most, row_counts[i]);
-  return aux_bytes(L, aux_blocks_per_layer((int)L, most), E);
+  return aux_bytes(L, aux_blocks_per_layer((int)L, most, (int)E), E);
 }
 
 PMOE_API int pmoe_aux_loss_forward(const void* const* logits, const int64_t* row_counts, int64_t L, int dtype,
@@ -1025,18 +1025,19 @@ PMOE_API int pmoe_aux_loss_forward(const void* const* logits, const int64_t* row
   int32_t* rows = cv.take<int32_t>(nb);
   double* col_p = cv.take<double>(E);
   int64_t* col_c = cv.take<int64_t>(E);
+  uint32_t* arrived = cv.take<uint32_t>(1);
   for (int64_t i = 0; i < L; i += kAuxMaxLayers) {
     const int n = (int)std::min<int64_t>(kAuxMaxLayers, L - i);
     const AuxLayers t = layer_table(logits, row_counts, i, n);
     const size_t b = (size_t)i * plan.bpl;
     hipError_t st = by_dtype16(dtype, [&](auto tp) {
       return aux_stats<PMOE_ELEM(tp)>(t, n, mask, (int)E, (int)K, plan.bpl, psum + b * E, counts + b * E, lse2 + b,
-                                      rows + b, s);
+                                      rows + b, arrived, s);
     });
     PMOE_TRY(st, "aux_loss_forward");
   }
   return hip_status(aux_finish(psum, counts, lse2, rows, (int)L, plan.bpl, (int)E, (int)K, aux_coef, z_coef,
-                               expert_counts, col_p, col_c, AuxOut{loss, load_balance, z_loss, coef}, s),
+                               expert_counts, col_p, col_c, arrived, AuxOut{loss, load_balance, z_loss, coef}, s),
                     "aux_loss_forward");
 }
 

@@ -21,39 +21,114 @@
 namespace pmoe {
 namespace {
 
-constexpr int kBlock = 256;
-constexpr int kWaves = kBlock / kWave;
+constexpr int kBlock = 256;        // threads of a block: the gradient, the statistics' sums
+constexpr int kFinishBlock = 1024;  // of the second launch
+constexpr int64_t kAuxOneBlock = 1 << 16;  // partial sums up to which it has one block
+constexpr int kCols = 32;           // its experts a block where it has several blocks
+// Threads of a block of the forward's pass over the logits, by the columns a row is padded to: a
+// compute unit's worth of waves, as far as their sums fit LDS together.
+constexpr int stats_block(int cols) { return cols <= 256 ? 1024 : 256; }
 
-// The largest / the sum over the LPR lanes (consecutive, a power of two) of a row.
+// Lane l's value from another lane of its row by a DPP control (quad permutation, row mirrors).
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, true); }
+
+// The two halves' values of an exchange between lanes 16 or 32 apart, in both.
+__device__ __forceinline__ u32x2 swap16(int v) { return __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false); }
+__device__ __forceinline__ u32x2 swap32(int v) { return __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false); }
+
+// All-reduce over the LPR consecutive lanes of a row by `op`: pairs, quads, halves
+// of 8 and of 16 by DPP, then by lane swaps (no LDS traffic). At each step two
+// halves that agree within themselves are joined, so every lane ends with the
+// same bits.
+template <int LPR, class Op>
+__device__ __forceinline__ int row_reduce(int v, Op op) {
+  if constexpr (LPR >= 2) v = op(v, dpp<0xB1>(v));
+  if constexpr (LPR >= 4) v = op(v, dpp<0x4E>(v));
+  if constexpr (LPR >= 8) v = op(v, dpp<0x141>(v));   // lane i of 8 takes lane 7 - i
+  if constexpr (LPR >= 16) v = op(v, dpp<0x140>(v));  // lane i of 16 takes lane 15 - i
+  if constexpr (LPR >= 32) { const u32x2 r = swap16(v); v = op((int)r[0], (int)r[1]); }
+  if constexpr (LPR >= 64) { const u32x2 r = swap32(v); v = op((int)r[0], (int)r[1]); }
+  return v;
+}
+
+// The sum over a wave's lanes l, l + LPR, l + 2 LPR, .. (the same columns of its
+// rows), in lane l < LPR; order fixed.
+template <int LPR, class Op>
+__device__ __forceinline__ int across_rows(int v, Op op) {
+  if constexpr (LPR <= 8) v = op(v, dpp<0x128>(v));  // row_ror: lane i + 8 of 16
+  if constexpr (LPR <= 4) v = op(v, dpp<0x124>(v));
+  static_assert(LPR >= 4, "rows of four lanes or more");
+  if constexpr (LPR <= 16) { const u32x2 r = swap16(v); v = op((int)r[0], (int)r[1]); }
+  if constexpr (LPR <= 32) { const u32x2 r = swap32(v); v = op((int)r[0], (int)r[1]); }
+  return v;
+}
 template <int LPR>
 __device__ __forceinline__ uint32_t row_max(uint32_t v) {
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, kWave));
-  return v;
+  return (uint32_t)row_reduce<LPR>((int)v, [](int a, int b) { return (int)max((uint32_t)a, (uint32_t)b); });
+}
+template <int LPR>
+__device__ __forceinline__ uint32_t row_min(uint32_t v) {
+  return (uint32_t)row_reduce<LPR>((int)v, [](int a, int b) { return (int)min((uint32_t)a, (uint32_t)b); });
+}
+template <int LPR>
+__device__ __forceinline__ float row_fmax(float v) {
+  return __int_as_float(row_reduce<LPR>(__float_as_int(v), [](int a, int b) {
+    return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
+  }));
 }
 template <int LPR>
 __device__ __forceinline__ int row_add(int v) {
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) v += __shfl_xor(v, o, kWave);
-  return v;
+  return row_reduce<LPR>(v, [](int a, int b) { return a + b; });
 }
 template <int LPR>
 __device__ __forceinline__ float row_add(float v) {
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) v += __shfl_xor(v, o, kWave);
-  return v;
+  return __int_as_float(row_reduce<LPR>(__float_as_int(v), [](int a, int b) {
+    return __float_as_int(__int_as_float(a) + __int_as_float(b));
+  }));
 }
+
+// e^x for x <= 0 (or NaN) from the hardware exp2: x log2 e is rounded once, so the relative error is |x| 2^-24 and 1 ulp.
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
 // Unsigned keys in the order of the values: -0 and +0 alike, NaN above all
 // (torch's order). Every key is above 0, which stands for "no expert".
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const float y = x + 0.0f;  // -0 -> +0
-  const uint32_t u = y != y ? 0x7fc00000u : __float_as_uint(y);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-__device__ __forceinline__ float key_value(uint32_t k) {
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
+__device__ __forceinline__ uint32_t order_bits(uint32_t u) { return (u & 0x80000000u) ? ~u : (u | 0x80000000u); }
+__device__ __forceinline__ uint32_t value_bits(uint32_t k) { return (k & 0x80000000u) ? (k & 0x7fffffffu) : ~k; }
+
+// fp32: the value's own 32 bits; equal values have equal keys. 16 bits: the
+// value's 16 bits above, and below them the column counted down, so that all keys
+// of a row differ and equal values are in the order of their ids (16-bit logits
+// are often equal).
+template <typename T> struct Key {
+  static constexpr bool unique = false;
+  __device__ static __forceinline__ uint32_t of(float x, int) {
+    const float y = x + 0.0f;  // -0 -> +0
+    return order_bits(y != y ? 0x7fc00000u : __float_as_uint(y));
+  }
+  __device__ static __forceinline__ float value(uint32_t k) { return __uint_as_float(value_bits(k)); }
+};
+template <> struct Key<bf16_t> {
+  static constexpr bool unique = true;
+  __device__ static __forceinline__ uint32_t of(float x, int col) {
+    return (Key<float>::of(x, 0) & 0xffff0000u) | (0xffffu - (uint32_t)col);
+  }
+  __device__ static __forceinline__ float value(uint32_t k) {
+    return __uint_as_float(value_bits(k) & 0xffff0000u);
+  }
+};
+template <> struct Key<f16_t> {
+  static constexpr bool unique = true;
+  __device__ static __forceinline__ uint32_t of(float x, int col) {
+    const float y = x + 0.0f;
+    const uint32_t u = y != y ? 0x7e00u : (uint32_t)__builtin_bit_cast(uint16_t, (f16_t)y);
+    return (order_bits(u << 16) & 0xffff0000u) | (0xffffu - (uint32_t)col);
+  }
+  __device__ static __forceinline__ float value(uint32_t k) {
+    const uint32_t u = value_bits(k) >> 16;
+    return (float)__builtin_bit_cast(f16_t, (uint16_t)u);
+  }
+};
 
 // A row's columns in a lane: J pieces of W consecutive ones (W elements are one
 // load), piece j of lane l from column (j * LPR + l) * W.
@@ -107,12 +182,45 @@ struct Row {
   }
 };
 
-// Bit i of the result: the lane's value i is among the row's K largest. Each of
-// up to K steps takes the largest key below the last one with all its equals;
-// the step in which they no longer all fit takes the lowest ids of them. Keys 0
-// (columns past E) are never taken, K <= E.
+// The K-th largest of a row's distinct keys: each step takes the largest key
+// below the last one. key - m as an unsigned number is largest for the key just
+// below m (keys at or above m wrap to less), so a step is one subtraction a key
+// and the maximum.
+template <int LPR, int V>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[V], uint32_t top, int K) {
+  uint32_t m = top;
+  for (int k = 1; k < K; ++k) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t = max(t, key[i] - m);
+    m += row_max<LPR>(t);
+  }
+  return m;
+}
+
+// One above the K-th smallest of a row's keys, the smallest being 0, where the K
+// smallest are distinct: each step takes the smallest key from m on, key - m (keys
+// below m wrap to more). Where fewer than K distinct keys exist the result is of
+// no use, which the caller sees from how many keys lie below it.
+template <int LPR, int V>
+__device__ __forceinline__ uint32_t above_kth_smallest(const uint32_t (&key)[V], int K) {
+  uint32_t m = 1;
+  for (int k = 1; k < K; ++k) {
+    uint32_t t = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t = min(t, key[i] - m);
+    m += row_min<LPR>(t) + 1u;
+  }
+  return m;
+}
+
+// The selection where equal keys decide it. Bit i of the result: the lane's
+// value i is among the row's K largest. Each of up to K steps takes the largest
+// key below the last one with all its equals; the step in which they no longer
+// all fit takes the lowest ids of them. Keys 0 (columns past E) are never taken,
+// K <= E.
 template <int LPR, int V, int W>
-__device__ __forceinline__ uint32_t select_top(const uint32_t (&key)[V], uint32_t top, int K, int l) {
+__device__ __forceinline__ uint32_t select_ties(const uint32_t (&key)[V], uint32_t top, int K, int l) {
   uint32_t m = top;
   int left = K;
   bool done = false;
@@ -137,37 +245,41 @@ __device__ __forceinline__ uint32_t select_top(const uint32_t (&key)[V], uint32_
     int mine = 0;
 #pragma unroll
     for (int e = 0; e < W; ++e) mine += key[j * W + e] == m;
-    int below = 0, all = 0;  // equals of this piece in lower lanes, and in all lanes
+    int upto = mine;  // equals of this piece in lanes up to this one
 #pragma unroll
-    for (int o = 0; o < LPR; ++o) {
-      const int c = __shfl(mine, o, LPR);
-      below += o < l ? c : 0;
-      all += c;
+    for (int o = 1; o < LPR; o <<= 1) {
+      const int c = __shfl_up(upto, o, LPR);
+      upto += l >= o ? c : 0;
     }
-    int rank = before + below;
+    int rank = before + upto - mine;
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       const bool same = key[j * W + e] == m;
       if (key[j * W + e] > m || (same && rank < left)) sel |= 1u << (j * W + e);
       rank += same;
     }
-    before += all;
+    before += __shfl(upto, LPR - 1, LPR);
   }
   return sel;
 }
 
 // Partial sums over the rows of (layer blockIdx.y, block blockIdx.x of it):
-// psum[b][e], counts[b][e], lse2[b], rows[b], b = blockIdx.y * gridDim.x + blockIdx.x.
+// psum[b][e], counts[b][e], lse2[b], rows[b], b = blockIdx.y * gridDim.x +
+// blockIdx.x; clears `arrived` for the second launch.
 template <typename T, int LPR, int V, int W>
-__global__ __launch_bounds__(kBlock) void aux_stats_kernel(AuxLayers layers, const uint8_t* __restrict__ mask, int E,
-                                                           int K, float* __restrict__ psum, int32_t* __restrict__ counts,
-                                                           float* __restrict__ lse2, int32_t* __restrict__ rows) {
+__global__ __launch_bounds__(stats_block(LPR * V)) void aux_stats_kernel(AuxLayers layers, const uint8_t* __restrict__ mask,
+                                                                int E, int K, float* __restrict__ psum,
+                                                                int32_t* __restrict__ counts, float* __restrict__ lse2,
+                                                                int32_t* __restrict__ rows, uint32_t* arrived) {
   typedef Row<LPR, V, W> R;
   constexpr int RPW = kWave / LPR;  // rows of a wave
-  __shared__ float s_p[kWaves][LPR * V];
-  __shared__ int s_c[kWaves][LPR * V];
-  __shared__ float s_l[kWaves];
-  __shared__ int s_n[kWaves];
+  constexpr int NT = stats_block(LPR * V), NW = NT / kWave;
+  constexpr int PAD = LPR * V;
+  __shared__ float s_p[NW][PAD];
+  __shared__ int s_c[NW][PAD];
+  __shared__ float s_l[NW];
+  __shared__ int s_n[NW];
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *arrived = 0;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % LPR, sub = lane / LPR;
   const T* logits = static_cast<const T*>(layers.logits[blockIdx.y]);
   const int64_t N = layers.rows[blockIdx.y];
@@ -177,122 +289,146 @@ __global__ __launch_bounds__(kBlock) void aux_stats_kernel(AuxLayers layers, con
   for (int i = 0; i < V; ++i) { ps[i] = 0.0f; ct[i] = 0; }
   float l2 = 0.0f;
   int n = 0;
-  const int64_t step = (int64_t)gridDim.x * kWaves * RPW;
-  for (int64_t base = ((int64_t)blockIdx.x * kWaves + wave) * RPW; base < N; base += step) {  // uniform over the wave
+  const int64_t step = (int64_t)gridDim.x * NW * RPW;
+  for (int64_t base = ((int64_t)blockIdx.x * NW + wave) * RPW; base < N; base += step) {  // uniform over the wave
     const int64_t t = base + sub;
     const bool valid = t < N && (mask == nullptr || mask[t] != 0);
-    float v[V];
-    R::load(logits + (valid ? t : base) * E, l, E, 0.0f, v);
-    uint32_t key[V], top = 0;
+    const T* row = logits + (valid ? t : base) * E;
+    float v[V], mx, s = 0.0f;
+    uint32_t key[V];
+    if constexpr (Key<T>::unique) {
+      R::load(row, l, E, 0.0f, v);
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      key[i] = R::col(l, i) < E ? order_key(v[i]) : 0u;
-      top = max(top, key[i]);
-    }
-    top = row_max<LPR>(top);
-    const float mx = key_value(top);
-    const uint32_t sel = select_top<LPR, V, W>(key, top, K, l);
-    float s = 0.0f;
+      for (int i = 0; i < V; ++i) {
+        key[i] = R::col(l, i) < E ? Key<T>::of(v[i], R::col(l, i)) : 0u;
+        top = max(top, key[i]);
+      }
+      top = row_max<LPR>(top);
+      mx = Key<T>::value(top);
+      uint32_t kth = kth_largest<LPR, V>(key, top, K);
+      if (!valid) kth = 0xffffffffu;  // above every key
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      v[i] = key[i] != 0u ? expf(v[i] - mx) : 0.0f;
-      s += v[i];
+      for (int i = 0; i < V; ++i) {
+        ct[i] += key[i] >= kth;
+        v[i] = key[i] != 0u ? exp_neg(v[i] - mx) : 0.0f;
+        s += v[i];
+      }
+      s = row_add<LPR>(s);
+    } else {
+      // Keys: the bits of max - x, which are in order where max - x >= 0 is finite or
+      // infinite, and never put a smaller x first (the rounding of a difference is
+      // monotonic): if exactly K keys lie below a border, they are the K largest x.
+      R::load(row, l, E, -INFINITY, v);
+      mx = v[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) mx = fmaxf(mx, v[i]);
+      mx = row_fmax<LPR>(mx);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = mx - v[i];
+        key[i] = R::col(l, i) < E ? __float_as_uint(d) : 0xffffffffu;
+        v[i] = R::col(l, i) < E ? exp_neg(-d) : 0.0f;
+        s += v[i];
+      }
+      s = row_add<LPR>(s);
+      uint32_t border = above_kth_smallest<LPR, V>(key, K);
+      if (!valid) border = 0u;
+      int below = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int b = key[i] < border;
+        ct[i] += b;
+        below += b;
+      }
+      below = row_add<LPR>(below);
+      // equal keys at a row's K-th place, or NaN or +inf in it (then s is NaN): the wave's rows again, by exact keys and ids
+      if (__any(valid && (below != K || s != s))) {
+        float x[V];
+        uint32_t exact[V], top = 0;
+        R::load(row, l, E, 0.0f, x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          exact[i] = R::col(l, i) < E ? Key<T>::of(x[i], 0) : 0u;
+          top = max(top, exact[i]);
+        }
+        const uint32_t sel = select_ties<LPR, V, W>(exact, row_max<LPR>(top), K, l);
+        if (valid) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) ct[i] += (int)((sel >> i) & 1) - (int)(key[i] < border);
+        }
+      }
     }
-    s = row_add<LPR>(s);
     const float inv = 1.0f / s, lse = mx + logf(s);
     if (valid) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        ps[i] += v[i] * inv;
-        ct[i] += (sel >> i) & 1;
-      }
+      for (int i = 0; i < V; ++i) ps[i] += v[i] * inv;
       if (l == 0) { l2 += lse * lse; ++n; }
     }
   }
   // the wave's rows, then the block's waves, in a fixed order
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int o = LPR; o < kWave; o <<= 1) {
-      ps[i] += __shfl_xor(ps[i], o, kWave);
-      ct[i] += __shfl_xor(ct[i], o, kWave);
-    }
-  l2 = wave_sum(l2);
-  n = row_add<kWave>(n);
-  if (sub == 0) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
+  for (int i = 0; i < V; ++i) {
+    ps[i] = __int_as_float(across_rows<LPR>(__float_as_int(ps[i]), [](int a, int b) {
+      return __float_as_int(__int_as_float(a) + __int_as_float(b));
+    }));
+    ct[i] = across_rows<LPR>(ct[i], [](int a, int b) { return a + b; });
+    if (sub == 0) {
       s_p[wave][R::col(l, i)] = ps[i];
       s_c[wave][R::col(l, i)] = ct[i];
     }
   }
+  l2 = wave_sum(l2);
+  n = row_add<kWave>(n);
   if (lane == 0) { s_l[wave] = l2; s_n[wave] = n; }
   __syncthreads();
   const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-  for (int e = threadIdx.x; e < E; e += kBlock) {
-    float p = s_p[0][e];
-    int c = s_c[0][e];
+  for (int e = threadIdx.x; e < E; e += NT) {
+    float p = 0.0f;
+    int c = 0;
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) { p += s_p[k][e]; c += s_c[k][e]; }
+    for (int k = 0; k < NW; ++k) { p += s_p[k][e]; c += s_c[k][e]; }
     psum[b * E + e] = p;
     counts[b * E + e] = c;
   }
-  if (threadIdx.x == 0) {
-    lse2[b] = ((s_l[0] + s_l[1]) + s_l[2]) + s_l[3];
-    rows[b] = s_n[0] + s_n[1] + s_n[2] + s_n[3];
+  if (threadIdx.x == NT - 1) {
+    float a = 0.0f;
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) { a += s_l[k]; c += s_n[k]; }
+    lse2[b] = a;
+    rows[b] = c;
   }
 }
 
-// Sums of the partial rows for 16 experts a block: counts per layer, their
-// total and the probabilities' sum (16 groups of rows, joined in order).
-__global__ __launch_bounds__(kBlock) void aux_columns_kernel(const float* __restrict__ psum,
-                                                             const int32_t* __restrict__ part_counts, int L, int bpl,
-                                                             int E, int32_t* __restrict__ counts,
-                                                             double* __restrict__ col_p, int64_t* __restrict__ col_c) {
-  __shared__ double s_p[16][16];
-  __shared__ int64_t s_c[16][16];
-  const int q = threadIdx.x % 16, grp = threadIdx.x / 16, e = blockIdx.x * 16 + q;
-  double p = 0.0;
-  int64_t c = 0;
-  if (e < E) {
-    for (int b = grp; b < L * bpl; b += 16) p += psum[(int64_t)b * E + e];
-    for (int layer = grp; layer < L; layer += 16) {
-      int own = 0;
-      for (int b = 0; b < bpl; ++b) own += part_counts[((int64_t)layer * bpl + b) * E + e];
-      counts[(int64_t)layer * E + e] = own;
-      c += own;
-    }
-  }
-  s_p[grp][q] = p;
-  s_c[grp][q] = c;
-  __syncthreads();
-  if (grp != 0 || e >= E) return;
-  for (int k = 1; k < 16; ++k) { p += s_p[k][q]; c += s_c[k][q]; }
-  col_p[e] = p;
-  col_c[e] = c;
-}
-
+// The sum over a block of NT threads, in every thread (s: NT / 64 values).
+template <int NT>
 __device__ __forceinline__ double block_sum(double v, double* s) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  __syncthreads();
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
   double a = s[0];
-  for (int k = 1; k < kWaves; ++k) a += s[k];
-  __syncthreads();
+#pragma unroll
+  for (int k = 1; k < NT / kWave; ++k) a += s[k];
   return a;
 }
 
-// The three losses from the columns' sums, and what the backward takes: f_e and 1 / n.
+// The three losses from the columns' sums, and what the backward takes: f_e and
+// 1 / n. FAR: the sums come from other blocks (read past this compute unit's cache).
+template <int NT, bool FAR>
 __device__ __forceinline__ void finish(const double* col_p, const int64_t* col_c, int64_t n, double lse2, int E, int K,
                                        float a, float z, const AuxOut& out, double* s) {
   const double inv = n > 0 ? 1.0 / (double)n : 0.0;
   double lb = 0.0;
-  for (int e = threadIdx.x; e < E; e += kBlock) {
-    lb += (double)col_c[e] * inv * (col_p[e] * inv);
-    out.f[e] = (float)((double)(col_c[e] * E - (int64_t)K * n) * inv / (double)E);
+  for (int e = threadIdx.x; e < E; e += NT) {
+    const double p = FAR ? __hip_atomic_load(col_p + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : col_p[e];
+    const int64_t c = FAR ? __hip_atomic_load(col_c + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : col_c[e];
+    lb += (double)c * inv * (p * inv);
+    out.f[e] = (float)((double)(c * E - (int64_t)K * n) * inv / (double)E);
   }
-  lb = block_sum(lb, s) * (double)E;
+  lb = block_sum<NT>(lb, s) * (double)E;
   if (threadIdx.x != 0) return;
   const double zl = lse2 * inv;
   out.loss[0] = (float)((double)a * lb + (double)z * zl);
@@ -301,32 +437,118 @@ __device__ __forceinline__ void finish(const double* col_p, const int64_t* col_c
   out.f[E] = (float)inv;
 }
 
-__global__ __launch_bounds__(kBlock) void aux_finish_kernel(const double* __restrict__ col_p,
-                                                            const int64_t* __restrict__ col_c,
-                                                            const float* __restrict__ lse2,
-                                                            const int32_t* __restrict__ rows, int nb, int E, int K,
-                                                            float a, float z, AuxOut out) {
-  __shared__ double s[kWaves];
-  double n = 0.0, l2 = 0.0;
-  for (int b = threadIdx.x; b < nb; b += kBlock) {
-    n += rows[b];  // whole numbers below 2^53: exact
+// The second launch: a block sums the partial rows of `cols` experts (a power of
+// two of at least 32), 1024 / cols groups of rows joined in order. One block then
+// makes the losses; of several, the last to finish does.
+__global__ __launch_bounds__(kFinishBlock) void aux_finish_kernel(const float* __restrict__ psum,
+                                                                  const int32_t* __restrict__ part_counts,
+                                                                  const float* __restrict__ lse2,
+                                                                  const int32_t* __restrict__ rows, int L, int bpl,
+                                                                  int E, int K, int cols, float a, float z,
+                                                                  int32_t* __restrict__ counts, double* col_p,
+                                                                  int64_t* col_c, uint32_t* arrived, AuxOut out) {
+  __shared__ int s_c[kFinishBlock];  // a layer's counts where several groups share it: then L * cols < 1024
+  __shared__ double s_p[kFinishBlock];
+  __shared__ int64_t s_t[kFinishBlock];
+  __shared__ double s[kFinishBlock / kWave];
+  __shared__ double s_l2[kFinishBlock / kWave];
+  __shared__ int s_n[kFinishBlock / kWave];
+  __shared__ bool s_last;
+  const int groups = kFinishBlock / cols;
+  const int q = threadIdx.x & (cols - 1), grp = threadIdx.x / cols, e = blockIdx.x * cols + q;
+  // S groups share a layer, each S-th row of it (few layers), or a group has every groups-th layer (S = 1)
+  const int S = max(1, groups / L), sub = grp % S, lstep = groups / S;
+  double p = 0.0;
+  int64_t c = 0;
+  s_c[threadIdx.x] = 0;
+  __syncthreads();
+  if (e < E && sub < bpl) {
+    constexpr int U = 12;  // rows in flight
+    const int per = (bpl - sub + S - 1) / S;  // this thread's rows of a layer
+    int ll = grp / S, lj = 0;                 // the next row to load
+    int l = ll, j = 0, own = 0;               // the next row to add, its layer's count so far
+    while (l < L) {
+      float pv[U];
+      int cv[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        pv[u] = 0.0f;
+        cv[u] = 0;
+        if (ll < L) {
+          const int64_t at = ((int64_t)ll * bpl + sub + (int64_t)lj * S) * E + e;
+          pv[u] = psum[at];
+          cv[u] = part_counts[at];
+        }
+        if (++lj == per) { lj = 0; ll += lstep; }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (l < L) {
+          p += pv[u];
+          own += cv[u];
+          if (++j == per) {
+            if (S > 1) atomicAdd(&s_c[l * cols + q], own);  // whole numbers: any order
+            else counts[(int64_t)l * E + e] = own;
+            c += own;
+            own = j = 0;
+            l += lstep;
+          }
+        }
+      }
+    }
+  }
+  s_p[threadIdx.x] = p;
+  s_t[threadIdx.x] = c;
+  int n = 0;
+  double l2 = 0.0;
+  for (int b = threadIdx.x; b < L * bpl; b += kFinishBlock) {
+    n += rows[b];
     l2 += lse2[b];
   }
-  n = block_sum(n, s);
-  l2 = block_sum(l2, s);
-  finish(col_p, col_c, (int64_t)n, l2, E, K, a, z, out, s);
+  n = row_add<kWave>(n);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l2 += __shfl_xor(l2, o, kWave);
+  if ((threadIdx.x & 63) == 0) { s_n[threadIdx.x >> 6] = n; s_l2[threadIdx.x >> 6] = l2; }
+  __syncthreads();
+  n = 0;
+  l2 = 0.0;
+#pragma unroll
+  for (int k = 0; k < kFinishBlock / kWave; ++k) { n += s_n[k]; l2 += s_l2[k]; }
+  if (S > 1 && e < E && grp < L) counts[(int64_t)grp * E + e] = s_c[grp * cols + q];
+  const bool one = gridDim.x == 1;
+  if (grp == 0 && e < E) {
+    for (int k = 1; k < groups; ++k) { p += s_p[k * cols + q]; c += s_t[k * cols + q]; }
+    if (one) {
+      s_p[q] = p;
+      s_t[q] = c;
+    } else {
+      __hip_atomic_store(col_p + e, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(col_c + e, c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (one) {  // a column's sums are read by the thread that wrote them
+    finish<kFinishBlock, false>(s_p, s_t, n, l2, E, K, a, z, out, s);
+    return;
+  }
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(arrived, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  finish<kFinishBlock, true>(col_p, col_c, n, l2, E, K, a, z, out, s);
 }
 
 // The same from the statistics that the fused routers already have (one block).
 __global__ __launch_bounds__(kBlock) void aux_from_stats_kernel(AuxStats st, int L, int64_t n, int E, int K, float a,
-                                                                float z, int32_t* __restrict__ counts,
-                                                                double* __restrict__ col_p,
-                                                                int64_t* __restrict__ col_c, int first, int last,
-                                                                double* __restrict__ lse2_sum, AuxOut out) {
-  __shared__ double s[kWaves];
-  for (int e = threadIdx.x; e < E; e += kBlock) {  // each thread's own columns: read back below by the same thread
+                                                                float z, int32_t* __restrict__ counts, double* col_p,
+                                                                int64_t* col_c, int first, int last,
+                                                                double* lse2_sum, AuxOut out) {
+  __shared__ double s[kBlock / kWave];
+  for (int e = threadIdx.x; e < E; e += kBlock) {  // each thread's own columns: read back in finish() by the same thread
     double p = first ? 0.0 : col_p[e];
     int64_t c = first ? 0 : col_c[e];
+#pragma unroll 4
     for (int i = 0; i < L; ++i) {
       const int32_t k = st.counts[i][e];
       counts[(int64_t)i * E + e] = k;
@@ -338,10 +560,10 @@ __global__ __launch_bounds__(kBlock) void aux_from_stats_kernel(AuxStats st, int
   }
   double l2 = 0.0;
   for (int i = threadIdx.x; i < L; i += kBlock) l2 += st.lse_sq_sum[i][0];
-  l2 = block_sum(l2, s) + (first ? 0.0 : lse2_sum[0]);
+  l2 = block_sum<kBlock>(l2, s) + (first ? 0.0 : lse2_sum[0]);
   __syncthreads();
   if (threadIdx.x == 0) lse2_sum[0] = l2;
-  if (last) finish(col_p, col_c, n, l2, E, K, a, z, out, s);
+  if (last) finish<kBlock, false>(col_p, col_c, n, l2, E, K, a, z, out, s);
 }
 
 template <typename T, int LPR, int V, int W>
@@ -350,7 +572,7 @@ __global__ __launch_bounds__(kBlock) void aux_grad_kernel(AuxLayers layers, AuxG
                                                           const float* __restrict__ f, const float* __restrict__ dloss,
                                                           float a, float z) {
   typedef Row<LPR, V, W> R;
-  constexpr int RPW = kWave / LPR;
+  constexpr int RPW = kWave / LPR, kWaves = kBlock / kWave;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % LPR, sub = lane / LPR;
   const T* logits = static_cast<const T*>(layers.logits[blockIdx.y]);
   T* out = static_cast<T*>(grads.grad[blockIdx.y]);
@@ -376,12 +598,11 @@ __global__ __launch_bounds__(kBlock) void aux_grad_kernel(AuxLayers layers, AuxG
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < V; ++i) mx = fmaxf(mx, v[i]);
-#pragma unroll
-    for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, kWave));
+    mx = row_fmax<LPR>(mx);
     float s = 0.0f, d = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      v[i] = R::col(l, i) < E ? expf(v[i] - mx) : 0.0f;
+      v[i] = R::col(l, i) < E ? exp_neg(v[i] - mx) : 0.0f;
       s += v[i];
       d += v[i] * fe[i];
     }
@@ -426,29 +647,36 @@ uintptr_t low_bits(const AuxLayers& a, const AuxGrads* g, int L) {
 
 }  // namespace
 
-// Blocks of one layer: about kAuxBlocks in all, each with at least 64 rows.
-int aux_blocks_per_layer(int L, int64_t max_rows) {
-  const int64_t want = std::max(1, kAuxBlocks / std::max(1, L));
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (max_rows + 63) / 64));
+// Blocks of one layer: a block a compute unit in all (two where there are more
+// layers than let that come out even, or blocks are small), each with rows for
+// all its waves.
+int aux_blocks_per_layer(int L, int64_t max_rows, int E) {
+  const bool small = stats_block(E) < 1024;
+  const int blocks = small || L > kAuxMaxLayers ? 2 * kAuxBlocks : kAuxBlocks;
+  const int64_t want = L <= kAuxMaxLayers ? blocks / std::max(1, L) : (blocks + L - 1) / L;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (max_rows + (small ? 15 : 63)) / (small ? 16 : 64)));
 }
 
 template <typename T>
 hipError_t aux_stats(const AuxLayers& layers, int L, const uint8_t* mask, int E, int K, int bpl, float* psum,
-                     int32_t* counts, float* lse2, int32_t* rows, hipStream_t s) {
+                     int32_t* counts, float* lse2, int32_t* rows, uint32_t* arrived, hipStream_t s) {
   return by_experts<T>(E, low_bits(layers, nullptr, L), [&](auto lpr, auto v, auto w) {
     hipLaunchKernelGGL((aux_stats_kernel<T, decltype(lpr)::value, decltype(v)::value, decltype(w)::value>),
-                       dim3(bpl, L), dim3(kBlock), 0, s, layers, mask, E, K, psum, counts, lse2, rows);
+                       dim3(bpl, L), dim3(stats_block(decltype(lpr)::value * decltype(v)::value)), 0, s, layers, mask, E, K, psum, counts, lse2, rows, arrived);
     return hipGetLastError();
   });
 }
 
 hipError_t aux_finish(const float* psum, const int32_t* part_counts, const float* lse2, const int32_t* rows, int L,
                       int bpl, int E, int K, float a, float z, int32_t* counts, double* col_p, int64_t* col_c,
-                      const AuxOut& out, hipStream_t s) {
-  hipLaunchKernelGGL(aux_columns_kernel, dim3((E + 15) / 16), dim3(kBlock), 0, s, psum, part_counts, L, bpl, E, counts,
-                     col_p, col_c);
-  hipLaunchKernelGGL(aux_finish_kernel, dim3(1), dim3(kBlock), 0, s, col_p, col_c, lse2, rows, L * bpl, E, K, a, z,
-                     out);
+                      uint32_t* arrived, const AuxOut& out, hipStream_t s) {
+  // one block while it reads the partial sums in a few microseconds; several need
+  // device-wide fences between them
+  int cols = kCols;
+  if (E <= 256 && (int64_t)L * bpl * E <= kAuxOneBlock)
+    while (cols < E) cols *= 2;
+  hipLaunchKernelGGL(aux_finish_kernel, dim3((E + cols - 1) / cols), dim3(kFinishBlock), 0, s, psum, part_counts,
+                     lse2, rows, L, bpl, E, K, cols, a, z, counts, col_p, col_c, arrived, out);
   return hipGetLastError();
 }
 
@@ -464,7 +692,7 @@ template <typename T>
 hipError_t aux_grad(const AuxLayers& layers, const AuxGrads& grads, int L, int64_t max_rows, const uint8_t* mask,
                     int E, const float* f, const float* dloss, float a, float z, hipStream_t s) {
   return by_experts<T>(E, low_bits(layers, &grads, L), [&](auto lpr, auto v, auto w) {
-    constexpr int RPB = kWaves * (kWave / decltype(lpr)::value);
+    constexpr int RPB = kBlock / decltype(lpr)::value;
     const int64_t want = std::max(1, 4096 / std::max(1, L));
     const int bpl = (int)std::max<int64_t>(1, std::min<int64_t>(want, (max_rows + RPB - 1) / RPB));
     hipLaunchKernelGGL((aux_grad_kernel<T, decltype(lpr)::value, decltype(v)::value, decltype(w)::value>),
@@ -475,7 +703,7 @@ hipError_t aux_grad(const AuxLayers& layers, const AuxGrads& grads, int L, int64
 
 #define PMOE_INST_AUX(T)                                                                                             \
   template hipError_t aux_stats<T>(const AuxLayers&, int, const uint8_t*, int, int, int, float*, int32_t*, float*,   \
-                                   int32_t*, hipStream_t);                                                           \
+                                   int32_t*, uint32_t*, hipStream_t);                                                           \
   template hipError_t aux_grad<T>(const AuxLayers&, const AuxGrads&, int, int64_t, const uint8_t*, int,              \
                                   const float*, const float*, float, float, hipStream_t);
 PMOE_INST_AUX(float)

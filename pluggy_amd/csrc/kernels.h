@@ -173,7 +173,7 @@ hipError_t act8_restore_swiglu(const int8_t* codes, const uint8_t* exps, const f
 
 // ---- the router's auxiliary loss (aux_loss.hip). Up to kAuxMaxLayers layers a launch.
 constexpr int kAuxMaxLayers = 64;
-constexpr int kAuxBlocks = 512;
+constexpr int kAuxBlocks = 256;
 struct AuxLayers { const void* logits[kAuxMaxLayers]; int64_t rows[kAuxMaxLayers]; };
 struct AuxGrads { void* grad[kAuxMaxLayers]; };
 struct AuxStats {
@@ -182,15 +182,15 @@ struct AuxStats {
   const float* lse_sq_sum[kAuxMaxLayers];
 };
 struct AuxOut { float* loss; float* balance; float* z; float* f; };  // f: E + 1 floats for aux_grad (f_e and 1 / n)
-int aux_blocks_per_layer(int L, int64_t max_rows);
-// Partial sums of L * bpl blocks: psum and counts (L * bpl, E), lse2 and rows (L * bpl).
+int aux_blocks_per_layer(int L, int64_t max_rows, int E);
+// Partial sums of L * bpl blocks: psum and counts (L * bpl, E), lse2 and rows (L * bpl); arrived: aux_finish's counter.
 template <typename T>
 hipError_t aux_stats(const AuxLayers& layers, int L, const uint8_t* mask, int E, int K, int bpl, float* psum,
-                     int32_t* counts, float* lse2, int32_t* rows, hipStream_t s);
+                     int32_t* counts, float* lse2, int32_t* rows, uint32_t* arrived, hipStream_t s);
 // counts (L, E); col_p, col_c: E each.
 hipError_t aux_finish(const float* psum, const int32_t* part_counts, const float* lse2, const int32_t* rows, int L,
                       int bpl, int E, int K, float a, float z, int32_t* counts, double* col_p, int64_t* col_c,
-                      const AuxOut& out, hipStream_t s);
+                      uint32_t* arrived, const AuxOut& out, hipStream_t s);
 hipError_t aux_from_stats(const AuxStats& st, int L, int64_t n, int E, int K, float a, float z, int32_t* counts,
                           double* col_p, int64_t* col_c, bool first, bool last, double* lse2_sum, const AuxOut& out,
                           hipStream_t s);
