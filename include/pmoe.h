@@ -378,7 +378,7 @@ PMOE_API int pmoe_aux_loss_backward(const void* const* logits, void* const* grad
  * arithmetic. x (T,H) x_dtype; weight and bias (H,) w_dtype or NULL (1 and 0);
  * out (T,H) out_dtype: x_dtype, or 16 bits from fp32 x; mean and rstd (T,) fp32,
  * or both NULL. Any H >= 1 (rows of 16-byte pieces are read as such, others
- * element by element); T < 2^24. */
+ * element by element); T < 2^23. */
 PMOE_API int pmoe_layernorm_forward(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype,
                                     float eps, int64_t T, int64_t H, void* out, int out_dtype, float* mean,
                                     float* rstd, void* stream);

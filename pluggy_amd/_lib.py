@@ -136,8 +136,15 @@ def ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+try:  # the handle alone; torch.cuda.current_stream builds a Stream object around it (2 us a call)
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 def stream_of(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.device.index)
 
 
 def require_gpu(*tensors: torch.Tensor) -> None:

@@ -1108,7 +1108,7 @@ PMOE_API int pmoe_aux_loss_backward(const void* const* logits, void* const* grad
 extern "C++" {
 namespace {
 
-constexpr int64_t kLnMaxRows = ((int64_t)1 << 24) - 1;  // 256 threads a row, below 2^32 a launch
+constexpr int64_t kLnMaxRows = ((int64_t)1 << 23) - 1;  // 512 threads a row, below 2^32 a launch
 
 int check_layernorm(int64_t T, int64_t H, int x_dtype, int w_dtype, int y_dtype, const char* what) {
   PMOE_REQUIRE(T >= 0 && H > 0 && H <= (int64_t)1 << 30, "%s: bad sizes T=%lld H=%lld", what, (long long)T,

@@ -17,6 +17,7 @@
 // rows, which a second launch sums: no floating atomics, so the same inputs
 // give the same bits.
 #include "kernels.h"
+#include "lanes.h"
 
 namespace pmoe {
 namespace {
@@ -29,65 +30,20 @@ constexpr int kCols = 32;           // its experts a block where it has several 
 // compute unit's worth of waves, as far as their sums fit LDS together.
 constexpr int stats_block(int cols) { return cols <= 256 ? 1024 : 256; }
 
-// Lane l's value from another lane of its row by a DPP control (quad permutation, row mirrors).
-template <int CTRL>
-__device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, true); }
-
-// The two halves' values of an exchange between lanes 16 or 32 apart, in both.
-__device__ __forceinline__ u32x2 swap16(int v) { return __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false); }
-__device__ __forceinline__ u32x2 swap32(int v) { return __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false); }
-
-// All-reduce over the LPR consecutive lanes of a row by `op`: pairs, quads, halves
-// of 8 and of 16 by DPP, then by lane swaps (no LDS traffic). At each step two
-// halves that agree within themselves are joined, so every lane ends with the
-// same bits.
-template <int LPR, class Op>
-__device__ __forceinline__ int row_reduce(int v, Op op) {
-  if constexpr (LPR >= 2) v = op(v, dpp<0xB1>(v));
-  if constexpr (LPR >= 4) v = op(v, dpp<0x4E>(v));
-  if constexpr (LPR >= 8) v = op(v, dpp<0x141>(v));   // lane i of 8 takes lane 7 - i
-  if constexpr (LPR >= 16) v = op(v, dpp<0x140>(v));  // lane i of 16 takes lane 15 - i
-  if constexpr (LPR >= 32) { const u32x2 r = swap16(v); v = op((int)r[0], (int)r[1]); }
-  if constexpr (LPR >= 64) { const u32x2 r = swap32(v); v = op((int)r[0], (int)r[1]); }
-  return v;
-}
-
-// The sum over a wave's lanes l, l + LPR, l + 2 LPR, .. (the same columns of its
-// rows), in lane l < LPR; order fixed.
-template <int LPR, class Op>
-__device__ __forceinline__ int across_rows(int v, Op op) {
-  if constexpr (LPR <= 8) v = op(v, dpp<0x128>(v));  // row_ror: lane i + 8 of 16
-  if constexpr (LPR <= 4) v = op(v, dpp<0x124>(v));
-  static_assert(LPR >= 4, "rows of four lanes or more");
-  if constexpr (LPR <= 16) { const u32x2 r = swap16(v); v = op((int)r[0], (int)r[1]); }
-  if constexpr (LPR <= 32) { const u32x2 r = swap32(v); v = op((int)r[0], (int)r[1]); }
-  return v;
-}
 template <int LPR>
 __device__ __forceinline__ uint32_t row_max(uint32_t v) {
-  return (uint32_t)row_reduce<LPR>((int)v, [](int a, int b) { return (int)max((uint32_t)a, (uint32_t)b); });
+  return (uint32_t)lanes_reduce<LPR>((int)v, [](int a, int b) { return (int)max((uint32_t)a, (uint32_t)b); });
 }
 template <int LPR>
 __device__ __forceinline__ uint32_t row_min(uint32_t v) {
-  return (uint32_t)row_reduce<LPR>((int)v, [](int a, int b) { return (int)min((uint32_t)a, (uint32_t)b); });
+  return (uint32_t)lanes_reduce<LPR>((int)v, [](int a, int b) { return (int)min((uint32_t)a, (uint32_t)b); });
 }
 template <int LPR>
 __device__ __forceinline__ float row_fmax(float v) {
-  return __int_as_float(row_reduce<LPR>(__float_as_int(v), [](int a, int b) {
+  return __int_as_float(lanes_reduce<LPR>(__float_as_int(v), [](int a, int b) {
     return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
   }));
 }
-template <int LPR>
-__device__ __forceinline__ int row_add(int v) {
-  return row_reduce<LPR>(v, [](int a, int b) { return a + b; });
-}
-template <int LPR>
-__device__ __forceinline__ float row_add(float v) {
-  return __int_as_float(row_reduce<LPR>(__float_as_int(v), [](int a, int b) {
-    return __float_as_int(__int_as_float(a) + __int_as_float(b));
-  }));
-}
-
 // e^x for x <= 0 (or NaN) from the hardware exp2: x log2 e is rounded once, so the relative error is |x| 2^-24 and 1 ulp.
 __device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
@@ -232,7 +188,7 @@ __device__ __forceinline__ uint32_t select_ties(const uint32_t (&key)[V], uint32
       eq += key[i] == m;
       t = max(t, key[i] < m ? key[i] : 0u);
     }
-    eq = row_add<LPR>(eq);
+    eq = lanes_sum<LPR>(eq);
     t = row_max<LPR>(t);
     done = done || eq >= left;
     if (!done) { left -= eq; m = t; }
@@ -314,7 +270,7 @@ __global__ __launch_bounds__(stats_block(LPR * V)) void aux_stats_kernel(AuxLaye
         v[i] = key[i] != 0u ? exp_neg(v[i] - mx) : 0.0f;
         s += v[i];
       }
-      s = row_add<LPR>(s);
+      s = lanes_sum<LPR>(s);
     } else {
       // Keys: the bits of max - x, which are in order where max - x >= 0 is finite or
       // infinite, and never put a smaller x first (the rounding of a difference is
@@ -331,7 +287,7 @@ __global__ __launch_bounds__(stats_block(LPR * V)) void aux_stats_kernel(AuxLaye
         v[i] = R::col(l, i) < E ? exp_neg(-d) : 0.0f;
         s += v[i];
       }
-      s = row_add<LPR>(s);
+      s = lanes_sum<LPR>(s);
       uint32_t border = above_kth_smallest<LPR, V>(key, K);
       if (!valid) border = 0u;
       int below = 0;
@@ -341,7 +297,7 @@ __global__ __launch_bounds__(stats_block(LPR * V)) void aux_stats_kernel(AuxLaye
         ct[i] += b;
         below += b;
       }
-      below = row_add<LPR>(below);
+      below = lanes_sum<LPR>(below);
       // equal keys at a row's K-th place, or NaN or +inf in it (then s is NaN): the wave's rows again, by exact keys and ids
       if (__any(valid && (below != K || s != s))) {
         float x[V];
@@ -369,17 +325,15 @@ __global__ __launch_bounds__(stats_block(LPR * V)) void aux_stats_kernel(AuxLaye
   // the wave's rows, then the block's waves, in a fixed order
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    ps[i] = __int_as_float(across_rows<LPR>(__float_as_int(ps[i]), [](int a, int b) {
-      return __float_as_int(__int_as_float(a) + __int_as_float(b));
-    }));
-    ct[i] = across_rows<LPR>(ct[i], [](int a, int b) { return a + b; });
+    ps[i] = __int_as_float(lanes_across<LPR>(__float_as_int(ps[i]), AddF()));
+    ct[i] = lanes_across<LPR>(ct[i], AddI());
     if (sub == 0) {
       s_p[wave][R::col(l, i)] = ps[i];
       s_c[wave][R::col(l, i)] = ct[i];
     }
   }
-  l2 = wave_sum(l2);
-  n = row_add<kWave>(n);
+  l2 = lanes_sum<kWave>(l2);
+  n = lanes_sum<kWave>(n);
   if (lane == 0) { s_l[wave] = l2; s_n[wave] = n; }
   __syncthreads();
   const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
@@ -505,7 +459,7 @@ __global__ __launch_bounds__(kFinishBlock) void aux_finish_kernel(const float* _
     n += rows[b];
     l2 += lse2[b];
   }
-  n = row_add<kWave>(n);
+  n = lanes_sum<kWave>(n);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l2 += __shfl_xor(l2, o, kWave);
   if ((threadIdx.x & 63) == 0) { s_n[threadIdx.x >> 6] = n; s_l2[threadIdx.x >> 6] = l2; }
@@ -606,9 +560,9 @@ __global__ __launch_bounds__(kBlock) void aux_grad_kernel(AuxLayers layers, AuxG
       s += v[i];
       d += v[i] * fe[i];
     }
-    s = row_add<LPR>(s);
+    s = lanes_sum<LPR>(s);
     const float inv = 1.0f / s, lse = mx + logf(s);
-    const float mean_f = row_add<LPR>(d) * inv, zl = cz * lse;
+    const float mean_f = lanes_sum<LPR>(d) * inv, zl = cz * lse;
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = v[i] * inv * (ca * (fe[i] - mean_f) + zl);
     R::store(out + t * E, l, E, v);

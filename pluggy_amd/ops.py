@@ -393,31 +393,43 @@ def _pointers(tensors):
     return (ctypes.c_void_p * len(tensors))(*(0 if t is None else t.data_ptr() for t in tensors))
 
 
-def _layer_args(logits, mask):
-    """(pointers, rows, L, dtype code, mask pointer, mask rows, E) of the layers' logits, one dtype and device."""
-    require_gpu(mask, *logits)
-    E, dt = logits[0].shape[1], logits[0].dtype
-    assert all(t.dim() == 2 and t.shape[1] == E and t.dtype == dt and t.is_contiguous()
-               and t.device == logits[0].device for t in logits)
-    if mask is not None:
-        assert mask.dtype in (torch.bool, torch.uint8) and mask.dim() == 1 and mask.is_contiguous()
-        assert mask.device == logits[0].device
-    rows = (ctypes.c_int64 * len(logits))(*(t.shape[0] for t in logits))
-    return (_pointers(logits), rows, len(logits), dtype_code(dt), ptr(mask), 0 if mask is None else mask.shape[0], E)
+class _Layers:
+    """The layers' logits as the entry points take them: one dtype, device and number of experts, contiguous."""
+
+    def __init__(self, logits, mask):
+        require_gpu(mask, *logits)
+        first = logits[0]
+        E = first.shape[1]
+        shapes = [t.shape for t in logits]
+        assert all(len(s) == 2 and s[1] == E for s in shapes), f"logits of one width, got {shapes}"
+        assert len({t.dtype for t in logits}) == 1 and len({t.device for t in logits}) == 1
+        assert all([t.is_contiguous() for t in logits])
+        mask_rows = 0
+        if mask is not None:
+            assert mask.dtype in (torch.bool, torch.uint8) and mask.dim() == 1 and mask.is_contiguous()
+            assert mask.device == first.device
+            mask_rows = mask.shape[0]
+        self.rows = [s[0] for s in shapes]
+        self.L, self.E, self.dtype, self.device = len(logits), E, first.dtype, first.device
+        self.row_array = (ctypes.c_int64 * self.L)(*self.rows)
+        self.tail = (self.row_array, self.L, dtype_code(first.dtype), ptr(mask), mask_rows, E)
 
 
 def aux_loss_forward(logits, top_k: int, aux_coef: float, z_coef: float, mask=None):
     """The layers' logits, a list of (N_i, E) -> loss, load balance and z-loss (() fp32), expert_counts
     (L, E) int32, coef (E + 1,) fp32 for ``aux_loss_backward``. mask (N,) bool or uint8: rows that count."""
-    ptrs, rows, L, code, mask_ptr, mask_rows, E = _layer_args(logits, mask)
-    dev = logits[0].device
-    losses = tuple(torch.empty((), dtype=torch.float32, device=dev) for _ in range(3))
+    return _aux_loss_forward(_Layers(logits, mask), logits, top_k, aux_coef, z_coef)
+
+
+def _aux_loss_forward(layers, logits, top_k, aux_coef, z_coef):
+    dev, L, E = layers.device, layers.L, layers.E
+    losses = [torch.empty((), dtype=torch.float32, device=dev) for _ in range(3)]
     counts = torch.empty(L, E, dtype=torch.int32, device=dev)
     coef = torch.empty(E + 1, dtype=torch.float32, device=dev)
-    ws = workspace(size("pmoe_aux_loss_forward_workspace_size", rows, L, E), dev)
+    ws = workspace(size("pmoe_aux_loss_forward_workspace_size", layers.row_array, L, E), dev)
     with on_device(coef):
-        call("pmoe_aux_loss_forward", ptrs, rows, L, code, mask_ptr, mask_rows, E, top_k, aux_coef, z_coef,
-             *map(ptr, losses), ptr(counts), ptr(coef), ptr(ws), ws.numel(), stream_of(coef))
+        call("pmoe_aux_loss_forward", _pointers(logits), *layers.tail, top_k, aux_coef, z_coef, *map(ptr, losses),
+             ptr(counts), ptr(coef), ptr(ws), ws.numel(), stream_of(coef))
     return (*losses, counts, coef)
 
 
@@ -442,17 +454,24 @@ def aux_loss_from_stats(counts, prob_sums, lse_sq_sums, n: int, top_k: int, aux_
 def aux_loss_backward(logits, coef, grad_loss, aux_coef: float, z_coef: float, mask=None, needs=None):
     """-> every layer's gradient (N_i, E) in its logits' dtype (None where needs[i] is false); grad_loss:
     the loss's gradient, one fp32 value on the device."""
-    ptrs, rows, L, code, mask_ptr, mask_rows, E = _layer_args(logits, mask)
+    return _aux_loss_backward(_Layers(logits, mask), logits, coef, grad_loss, aux_coef, z_coef, needs)
+
+
+def _aux_loss_backward(layers, logits, coef, grad_loss, aux_coef, z_coef, needs=None):
     require_gpu(coef, grad_loss)
+    E = layers.E
     assert grad_loss.numel() == 1 and grad_loss.dtype == torch.float32 and coef.shape == (E + 1,)
     # one allocation for all layers; each gradient is its rows
-    need = [True] * L if needs is None else [bool(x) for x in needs]
-    sizes = [t.shape[0] if k else 0 for t, k in zip(logits, need)]
-    parts = torch.empty(sum(sizes), E, dtype=logits[0].dtype, device=logits[0].device).split(sizes)
-    grads = [g if k else None for g, k in zip(parts, need)]
+    if needs is None or all(needs):
+        sizes = layers.rows
+    else:
+        sizes = [n if k else 0 for n, k in zip(layers.rows, needs)]
+    grads = torch.empty(sum(sizes), E, dtype=layers.dtype, device=layers.device).split(sizes)
+    if sizes is not layers.rows:
+        grads = [g if k else None for g, k in zip(grads, needs)]
     with on_device(coef):
-        call("pmoe_aux_loss_backward", ptrs, _pointers(grads), rows, L, code, mask_ptr, mask_rows, E, ptr(coef),
-             ptr(grad_loss), aux_coef, z_coef, stream_of(coef))
+        call("pmoe_aux_loss_backward", _pointers(logits), _pointers(grads), *layers.tail, ptr(coef), ptr(grad_loss),
+             aux_coef, z_coef, stream_of(coef))
     return grads
 
 

@@ -144,16 +144,16 @@ class RouterAuxLoss:
 
 class _RouterAuxLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, top_k, aux_coef, z_coef, mask, stats, *logits):
+    def forward(ctx, layers, top_k, aux_coef, z_coef, mask, stats, *logits):
         with _stage("aux_loss"):
             if stats is None:
-                *losses, counts, coef = ops.aux_loss_forward(logits, top_k, aux_coef, z_coef, mask)
+                *losses, counts, coef = ops._aux_loss_forward(layers, logits, top_k, aux_coef, z_coef)
             else:
                 *losses, counts, coef = ops.aux_loss_from_stats(
                     [s.expert_counts for s in stats], [s.prob_sum for s in stats], [s.lse_sq_sum for s in stats],
                     sum(int(s.tokens) for s in stats), top_k, aux_coef, z_coef)
         ctx.save_for_backward(coef, mask, *logits)
-        ctx.coefs = (aux_coef, z_coef)
+        ctx.layers, ctx.coefs = layers, (aux_coef, z_coef)
         loss, balance, z = losses
         ctx.mark_non_differentiable(balance, z, counts)
         ctx.set_materialize_grads(False)
@@ -163,13 +163,18 @@ class _RouterAuxLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_loss, _gb, _gz, _gc):
         coef, mask, *logits = ctx.saved_tensors
-        needs = ctx.needs_input_grad[5:]
+        needs = ctx.needs_input_grad[6:]
         if g_loss is None or not any(needs):
-            return (None,) * (5 + len(logits))
+            return (None,) * (6 + len(logits))
         _refuse_capture("aux_loss_bwd")
+        # a saved-tensor hook may have given other tensors back: checked again unless they lie where they lay
+        layers = ctx.layers
+        if layers.tail[3] != ops.ptr(mask) or not all([t.is_contiguous() for t in logits]):
+            logits = [t.contiguous() for t in logits]
+            layers = ops._Layers(logits, mask)
         with _stage("aux_loss_bwd"):
-            grads = ops.aux_loss_backward(logits, coef, g_loss.float().contiguous(), *ctx.coefs, mask, needs)
-        return (None, None, None, None, None, *grads)
+            grads = ops._aux_loss_backward(layers, logits, coef, g_loss.float().contiguous(), *ctx.coefs, needs)
+        return (None, None, None, None, None, None, *grads)
 
 
 @torch.compiler.disable
@@ -203,9 +208,9 @@ def router_aux_loss(router_logits: list[torch.Tensor], num_experts: int, top_k: 
         zero = torch.tensor(0.0)
         return RouterAuxLoss(zero, zero, zero, torch.zeros(0, num_experts, dtype=torch.int32))
     assert 1 <= top_k <= num_experts
-    for lg in logits:
-        assert lg.dim() == 2 and lg.shape[1] == num_experts, f"router logits {tuple(lg.shape)}, expected (N, {num_experts})"
-        assert lg.dtype == logits[0].dtype and lg.device == logits[0].device, "logits of one type and device"
+    assert all(lg.dim() == 2 for lg in logits) and logits[0].shape[1] == num_experts, (
+        f"router logits {[tuple(lg.shape) for lg in logits]}, expected (N, {num_experts})")
+    assert len({lg.dtype for lg in logits}) == 1, f"router logits of one type, got {[lg.dtype for lg in logits]}"
     require_gpu(token_mask, *logits)
     mask = None
     if token_mask is not None:
@@ -218,9 +223,9 @@ def router_aux_loss(router_logits: list[torch.Tensor], num_experts: int, top_k: 
         assert len(stats) == len(logits) and all(int(s.tokens) == lg.shape[0] for s, lg in zip(stats, logits)), (
             "one RouterStats per layer's logits, of the same rows")
         assert all(s.expert_counts.shape == (num_experts,) for s in stats)
-    out = _RouterAuxLoss.apply(int(top_k), float(router_aux_loss_coef), float(router_z_loss_coef), mask, stats,
-                               *(lg.contiguous() for lg in logits))
-    return RouterAuxLoss(*out)
+    logits = [lg.contiguous() for lg in logits]
+    return RouterAuxLoss(*_RouterAuxLoss.apply(ops._Layers(logits, mask), int(top_k), float(router_aux_loss_coef),
+                                               float(router_z_loss_coef), mask, stats, *logits))
 
 
 def _sparse_routers(model):
