@@ -377,8 +377,8 @@ PMOE_API int pmoe_aux_loss_backward(const void* const* logits, void* const* grad
  * sqrt(mean((x[t] - mu)^2) + eps), out[t] = (x[t] - mu) r weight + bias, fp32
  * arithmetic. x (T,H) x_dtype; weight and bias (H,) w_dtype or NULL (1 and 0);
  * out (T,H) out_dtype: x_dtype, or 16 bits from fp32 x; mean and rstd (T,) fp32,
- * or both NULL. Any H >= 1 (rows of 16-byte pieces are read as such, others
- * element by element); T < 2^23. */
+ * or both NULL. Any H >= 1 and any alignment of the rows; T < 2^23 where
+ * H > 16384. */
 PMOE_API int pmoe_layernorm_forward(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype,
                                     float eps, int64_t T, int64_t H, void* out, int out_dtype, float* mean,
                                     float* rstd, void* stream);

@@ -1108,16 +1108,16 @@ PMOE_API int pmoe_aux_loss_backward(const void* const* logits, void* const* grad
 extern "C++" {
 namespace {
 
-constexpr int64_t kLnMaxRows = ((int64_t)1 << 23) - 1;  // 512 threads a row, below 2^32 a launch
 
 int check_layernorm(int64_t T, int64_t H, int x_dtype, int w_dtype, int y_dtype, const char* what) {
-  PMOE_REQUIRE(T >= 0 && H > 0 && H <= (int64_t)1 << 30, "%s: bad sizes T=%lld H=%lld", what, (long long)T,
-               (long long)H);
+  PMOE_REQUIRE(T >= 0 && T <= kMaxIndex && H > 0 && H <= (int64_t)1 << 30, "%s: bad sizes T=%lld H=%lld", what,
+               (long long)T, (long long)H);
   PMOE_REQUIRE(dtype16_ok(x_dtype) && dtype16_ok(w_dtype) && dtype16_ok(y_dtype), "unknown dtype code");
   PMOE_REQUIRE(y_dtype == x_dtype || x_dtype == PMOE_F32, "%s: the output has x's type, or 16 bits beside fp32 x",
                what);
-  if (T > kLnMaxRows)
-    return fail(PMOE_ERR_UNSUPPORTED, "%s: %lld rows > %lld", what, (long long)T, (long long)kLnMaxRows);
+  if (T > layernorm_max_rows((int)H))
+    return fail(PMOE_ERR_UNSUPPORTED, "%s: %lld rows of %lld columns exceed one launch", what, (long long)T,
+                (long long)H);
   return PMOE_OK;
 }
 
@@ -1150,7 +1150,7 @@ PMOE_API int pmoe_layernorm_forward(const void* x, int x_dtype, const void* weig
 }
 
 PMOE_API size_t pmoe_layernorm_backward_workspace_size(int64_t T, int64_t H) {
-  if (T <= 0 || T > kLnMaxRows || H <= 0 || H > (int64_t)1 << 30) return 0;
+  if (T <= 0 || H <= 0 || H > (int64_t)1 << 30 || T > layernorm_max_rows((int)H)) return 0;
   return align_up((size_t)2 * layernorm_bwd_blocks(T, (int)H) * layernorm_part_ld((int)H) * sizeof(float));
 }
 

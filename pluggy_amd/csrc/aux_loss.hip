@@ -249,11 +249,14 @@ __global__ __launch_bounds__(stats_block(LPR * V)) void aux_stats_kernel(AuxLaye
   for (int64_t base = ((int64_t)blockIdx.x * NW + wave) * RPW; base < N; base += step) {  // uniform over the wave
     const int64_t t = base + sub;
     const bool valid = t < N && (mask == nullptr || mask[t] != 0);
-    const T* row = logits + (valid ? t : base) * E;
+    // A lane past the end reads the wave's first row, and what it makes of it is not
+    // counted. (Reading the next rows ahead: 48 layers of 8192 x 128 62 -> 95 us, its
+    // registers do not fit four waves a SIMD; at 32 experts, where they do, no gain.)
+    const T* row = logits + (t < N ? t : base) * E;
     float v[V], mx, s = 0.0f;
+    R::load(row, l, E, Key<T>::unique ? 0.0f : -INFINITY, v);
     uint32_t key[V];
     if constexpr (Key<T>::unique) {
-      R::load(row, l, E, 0.0f, v);
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -275,7 +278,6 @@ __global__ __launch_bounds__(stats_block(LPR * V)) void aux_stats_kernel(AuxLaye
       // Keys: the bits of max - x, which are in order where max - x >= 0 is finite or
       // infinite, and never put a smaller x first (the rounding of a difference is
       // monotonic): if exactly K keys lie below a border, they are the K largest x.
-      R::load(row, l, E, -INFINITY, v);
       mx = v[0];
 #pragma unroll
       for (int i = 1; i < V; ++i) mx = fmaxf(mx, v[i]);
@@ -288,31 +290,29 @@ __global__ __launch_bounds__(stats_block(LPR * V)) void aux_stats_kernel(AuxLaye
         s += v[i];
       }
       s = lanes_sum<LPR>(s);
-      uint32_t border = above_kth_smallest<LPR, V>(key, K);
-      if (!valid) border = 0u;
+      const uint32_t border = above_kth_smallest<LPR, V>(key, K);
       int below = 0;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int b = key[i] < border;
-        ct[i] += b;
-        below += b;
-      }
+      for (int i = 0; i < V; ++i) below += key[i] < border;
       below = lanes_sum<LPR>(below);
       // equal keys at a row's K-th place, or NaN or +inf in it (then s is NaN): the wave's rows again, by exact keys and ids
       if (__any(valid && (below != K || s != s))) {
         float x[V];
-        uint32_t exact[V], top = 0;
         R::load(row, l, E, 0.0f, x);
+        uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          exact[i] = R::col(l, i) < E ? Key<T>::of(x[i], 0) : 0u;
-          top = max(top, exact[i]);
+          key[i] = R::col(l, i) < E ? Key<T>::of(x[i], 0) : 0u;
+          top = max(top, key[i]);
         }
-        const uint32_t sel = select_ties<LPR, V, W>(exact, row_max<LPR>(top), K, l);
+        const uint32_t sel = select_ties<LPR, V, W>(key, row_max<LPR>(top), K, l);
         if (valid) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) ct[i] += (int)((sel >> i) & 1) - (int)(key[i] < border);
+          for (int i = 0; i < V; ++i) ct[i] += (sel >> i) & 1;
         }
+      } else if (valid) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) ct[i] += key[i] < border;
       }
     }
     const float inv = 1.0f / s, lse = mx + logf(s);

@@ -160,6 +160,7 @@ hipError_t layernorm_bwd(const TG* g, const TX* x, const void* w, int w_code, co
                          int64_t T_, int H, TX* gx, float* part, void* gw, void* gb, hipStream_t s);
 int layernorm_bwd_blocks(int64_t T_, int H);
 int64_t layernorm_part_ld(int H);
+int64_t layernorm_max_rows(int H);
 
 // ---- activations saved in 8 bits (act8.hip; the format: act8.h). codes (R, C)
 // int8, exps (R, groups(C)) one byte a group; of gate_up rows (P, 2I): codes (P, 2I), exps (P, 2, groups(I)).

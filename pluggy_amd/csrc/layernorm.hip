@@ -481,6 +481,9 @@ int layernorm_bwd_blocks(int64_t T_, int H) {
 
 int64_t layernorm_part_ld(int H) { return ln_pad(H); }
 
+// Rows walked in passes have a block each: fewer than 2^32 threads a launch.
+int64_t layernorm_max_rows(int H) { return H > kLnRegH ? ((int64_t)1 << 32) / kLnBlock - 1 : 0x7fffffff; }
+
 template <typename TX, typename TO>
 hipError_t layernorm_fwd(const TX* x, const void* w, const void* b, int w_code, float eps, int64_t T_, int H, TO* out,
                          float* mean, float* rstd, hipStream_t s) {

@@ -354,7 +354,8 @@ def layernorm_forward(x, weight, bias, eps: float, out_dtype, stats: bool = True
     rstd (T,) fp32 (None without ``stats``). weight and bias (H,), one dtype, or None."""
     require_gpu(x, weight, bias)
     T, H = x.shape
-    assert x.is_contiguous() and all(p is None or (p.is_contiguous() and p.shape == (H,)) for p in (weight, bias))
+    assert x.is_contiguous() and all(p is None or (p.is_contiguous() and p.shape == (H,) and p.device == x.device)
+                                     for p in (weight, bias))
     assert weight is None or bias is None or weight.dtype == bias.dtype
     wdt = next((p.dtype for p in (weight, bias) if p is not None), torch.float32)
     out = torch.empty(T, H, dtype=out_dtype, device=x.device)
@@ -372,7 +373,8 @@ def layernorm_backward(grad, x, weight, mean, rstd, weight_dtype=torch.float32, 
     require_gpu(grad, x, weight, mean, rstd)
     T, H = x.shape
     assert grad.shape == x.shape and grad.is_contiguous() and x.is_contiguous()
-    assert weight is None or weight.dtype == weight_dtype
+    assert weight is None or (weight.dtype == weight_dtype and weight.shape == (H,) and weight.is_contiguous())
+    assert mean.shape == rstd.shape == (T,) and mean.dtype == rstd.dtype == torch.float32
     dev = x.device
     gx = torch.empty_like(x) if need_x else None
     gw = torch.empty(H, dtype=weight_dtype, device=dev) if need_weight else None
@@ -390,22 +392,26 @@ def layernorm_backward(grad, x, weight, mean, rstd, weight_dtype=torch.float32, 
 
 def _pointers(tensors):
     """A host array of the tensors' device pointers (None: a null one)."""
-    return (ctypes.c_void_p * len(tensors))(*(0 if t is None else t.data_ptr() for t in tensors))
+    return (ctypes.c_void_p * len(tensors))(*[0 if t is None else t.data_ptr() for t in tensors])
 
 
 class _Layers:
     """The layers' logits as the entry points take them: one dtype, device and number of experts, contiguous."""
 
     def __init__(self, logits, mask):
-        require_gpu(mask, *logits)
         first = logits[0]
-        E = first.shape[1]
         shapes = [t.shape for t in logits]
-        assert all(len(s) == 2 and s[1] == E for s in shapes), f"logits of one width, got {shapes}"
-        assert len({t.dtype for t in logits}) == 1 and len({t.device for t in logits}) == 1
+        E = shapes[0][-1]
+        assert all([len(s) == 2 and s[1] == E for s in shapes]), f"logits (N, E) of one E, got {shapes}"
+        assert len({t.dtype for t in logits}) == 1, f"logits of one type, got {[t.dtype for t in logits]}"
+        devices = {t.get_device() for t in logits}  # -1: not on a GPU
+        if devices != {first.get_device()} or -1 in devices:
+            require_gpu(*logits)
+            raise AssertionError(f"logits on one device, got {devices}")
         assert all([t.is_contiguous() for t in logits])
         mask_rows = 0
         if mask is not None:
+            require_gpu(mask)
             assert mask.dtype in (torch.bool, torch.uint8) and mask.dim() == 1 and mask.is_contiguous()
             assert mask.device == first.device
             mask_rows = mask.shape[0]
@@ -524,6 +530,7 @@ def gate_up_swiglu_act8(x, gate_up_proj, offs, row_index=None, row_weight=None):
     require_gpu(x, gate_up_proj, offs, row_index, row_weight)
     E, H, I = _dims(gate_up_proj)
     P = row_index.shape[0] if row_index is not None else x.shape[0]
+    assert x.shape[1] == H and x.dtype == gate_up_proj.dtype and x.is_contiguous() and gate_up_proj.is_contiguous()
     dev, code = x.device, dtype_code(x.dtype)
     codes = torch.empty(P, 2 * I, dtype=torch.int8, device=dev)
     exps = torch.empty(P, 2, act8_groups(I), dtype=torch.uint8, device=dev)
@@ -543,6 +550,8 @@ def down_proj_dgrad_act8(grad, codes, exps, down_proj_w, offs, row_index=None, r
     require_gpu(grad, down_proj_w, offs, row_index, row_weight)
     E, H, I = down_proj_w.shape
     P = row_index.shape[0] if row_index is not None else grad.shape[0]
+    assert grad.shape[1] == H and grad.dtype == down_proj_w.dtype
+    assert grad.is_contiguous() and down_proj_w.is_contiguous()
     assert codes.shape == (P, 2 * I) and exps.shape == (P, 2, act8_groups(I)), (
         f"codes {tuple(codes.shape)}, exps {tuple(exps.shape)} for P={P}, I={I}")
     dev, code = grad.device, dtype_code(grad.dtype)

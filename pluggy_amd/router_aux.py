@@ -208,13 +208,13 @@ def router_aux_loss(router_logits: list[torch.Tensor], num_experts: int, top_k: 
         zero = torch.tensor(0.0)
         return RouterAuxLoss(zero, zero, zero, torch.zeros(0, num_experts, dtype=torch.int32))
     assert 1 <= top_k <= num_experts
-    assert all(lg.dim() == 2 for lg in logits) and logits[0].shape[1] == num_experts, (
-        f"router logits {[tuple(lg.shape) for lg in logits]}, expected (N, {num_experts})")
-    assert len({lg.dtype for lg in logits}) == 1, f"router logits of one type, got {[lg.dtype for lg in logits]}"
-    require_gpu(token_mask, *logits)
+    assert logits[0].shape[-1] == num_experts, f"router logits {tuple(logits[0].shape)}, expected (N, {num_experts})"
+    if not all([lg.is_contiguous() for lg in logits]):
+        logits = [lg.contiguous() for lg in logits]
     mask = None
     if token_mask is not None:
         assert stats is None, "the statistics cover every row: token_mask needs the logits alone"
+        require_gpu(token_mask)
         assert not token_mask.is_floating_point() and all(lg.shape[0] == token_mask.numel() for lg in logits), (
             f"token_mask has {token_mask.numel()} entries, the layers {[lg.shape[0] for lg in logits]} rows")
         mask = token_mask if token_mask.dtype == torch.bool else token_mask != 0
@@ -222,8 +222,7 @@ def router_aux_loss(router_logits: list[torch.Tensor], num_experts: int, top_k: 
     if stats is not None:
         assert len(stats) == len(logits) and all(int(s.tokens) == lg.shape[0] for s, lg in zip(stats, logits)), (
             "one RouterStats per layer's logits, of the same rows")
-        assert all(s.expert_counts.shape == (num_experts,) for s in stats)
-    logits = [lg.contiguous() for lg in logits]
+        assert all(s.expert_counts.shape == (num_experts,) and s.expert_counts.device == logits[0].device for s in stats)
     return RouterAuxLoss(*_RouterAuxLoss.apply(ops._Layers(logits, mask), int(top_k), float(router_aux_loss_coef),
                                                float(router_z_loss_coef), mask, stats, *logits))
 

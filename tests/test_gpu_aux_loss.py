@@ -120,13 +120,14 @@ def test_coefficients(a, z):
 
 
 @pytest.mark.parametrize("E,K", [(8, 3), (32, 4), (128, 8), (130, 64), (1024, 5)])
-def test_ties_go_to_the_lower_id(E, K):
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+def test_ties_go_to_the_lower_id(E, K, dt):
     """All logits equal (a zero-initialised router), few distinct values, and zeros of both signs."""
     g = gen(E)
     same = torch.zeros(40, E)
     few = torch.randint(0, 3, (40, E), generator=g).float()
     signs = torch.where(torch.rand(40, E, generator=g) < 0.5, 0.0, -0.0)
-    logits = [t.to(DEV).requires_grad_() for t in (same, few, signs)]
+    logits = [t.to(DT[dt]).to(DEV).requires_grad_() for t in (same, few, signs)]
     r, grads = run(logits, K, 1.0, 0.1)
     check(r, grads, reference([t.abs() if i == 2 else t for i, t in enumerate(logits)], K, 1.0, 0.1), 1.0, 0.1)
     assert r.expert_counts[0, :K].eq(40).all() and r.expert_counts[0, K:].eq(0).all()
@@ -336,6 +337,55 @@ def test_losses_can_be_changed_in_place():
     total += 1.0
     total.backward()
     assert logits[0].grad is not None
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+def test_values_far_apart_and_close_together(dt):
+    """Rows whose maximum is so far above the rest that differences from it lose digits (equal after the
+    subtraction, not before), rows of neighbours in the type, and infinities on both ends of the order."""
+    E, K = 48, 5
+    g = gen(21)
+    eps = torch.finfo(DT[dt]).eps
+    far = torch.randn(60, E, generator=g) * 1e-3
+    far[torch.arange(60), torch.randint(0, E, (60,), generator=g)] = 1e4
+    near = 1.0 + eps * torch.randint(0, 9, (60, E), generator=g).float()
+    low = torch.randn(60, E, generator=g)
+    low[torch.rand(60, E, generator=g) < 0.8] = float("-inf")
+    low[:, 0] = 0.25
+    logits = [t.to(DT[dt]).to(DEV).requires_grad_() for t in (far, near, low)]
+    r, _ = run(logits, K, 1.0, 0.0)
+    assert torch.equal(r.expert_counts.cpu().long(), reference(logits, K, 1.0, 0.0)["counts"])
+
+
+def test_inside_a_compiled_function():
+    logits = draw(2, 60, 16, "fp32", 22)
+    import pluggy_amd
+
+    def f(a, b):
+        return pluggy_amd.router_aux_loss([a * 2, b * 2], 16, 2, 1.0, 0.1).loss * 3
+
+    want = f(*logits)
+    got = torch.compile(f, backend="aot_eager")(*logits)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, logits), torch.autograd.grad(want, logits)):
+        assert torch.equal(a, b)
+
+
+def test_gradients_under_saved_tensor_hooks():
+    """Hooks that give other tensors back (as activation offloading does), strided ones among them."""
+    logits = draw(3, 40, 12, "fp32", 23)
+    mask = torch.rand(40, generator=gen(23)) < 0.7
+    r, want = run(logits, 3, 1.0, 0.5, mask.to(DEV))
+    import pluggy_amd
+
+    def unpack(t):
+        t = t.clone()
+        return t.t().contiguous().t() if t.dim() == 2 else t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        r = pluggy_amd.router_aux_loss(logits, 12, 3, 1.0, 0.5, token_mask=mask.to(DEV))
+    for a, b in zip(torch.autograd.grad(r.loss, logits), want):
+        assert torch.equal(a, b)
 
 
 def test_forward_in_a_graph():

@@ -164,6 +164,42 @@ def test_shapes_strides_and_alignment():
     assert pluggy_amd.layer_norm(x[5], w, b).shape == (200,) and torch.equal(pluggy_amd.layer_norm(x[5], w, b), y[5])
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("H", [5, 127, 1000, 2047, 4095, 8191, 16383])
+def test_rows_at_any_alignment(dt, H):
+    """Rows, parameters and gradients that start on any element, and widths whose last chunk is cut."""
+    import pluggy_amd
+
+    T = 21
+    x, w, b, g = inputs(T, H, DT[dt], torch.float32, H)
+    g = g.to(DT[dt])
+
+    def shifted(t, by):
+        out = torch.zeros(t.numel() + by, dtype=t.dtype, device=DEV)[by:].view(t.shape)
+        return out.copy_(t)
+
+    leaves = [shifted(x, 3).requires_grad_(), shifted(w, 1).requires_grad_(), shifted(b, 2).requires_grad_()]
+    y = pluggy_amd.layer_norm(*leaves)
+    ref = reference(x, w, b, 1e-5, g, T, H)
+    check("y", y.detach(), *ref["y"])
+    for name, got in zip(("gx", "gw", "gb"), torch.autograd.grad(y, leaves, shifted(g, 1))):
+        check(name, got, *ref[name])
+
+
+@pytest.mark.parametrize("T,H", [(100003, 8), (70000, 40), (3000, 1024)])
+def test_many_rows(T, H):
+    """More rows than the grid has at a time."""
+    import pluggy_amd
+
+    x, w, b, g = inputs(T, H, torch.float32, torch.float32, H)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = pluggy_amd.layer_norm(*leaves)
+    ref = reference(x.detach(), w.detach(), b.detach(), 1e-5, g, T, H)
+    check("y", y.detach(), *ref["y"])
+    for name, got in zip(("gx", "gw", "gb"), torch.autograd.grad(y, leaves, g)):
+        check(name, got, *ref[name])
+
+
 def test_no_rows():
     import pluggy_amd
 

@@ -86,7 +86,8 @@ def norm_fwd(lib, T=4, H=8, x=0, w=0, y=0, eps=1e-5, px=FAKE, mean=None, rstd=No
     ({"T": -1}, -1, "sizes"),
     ({"H": 0}, -1, "sizes"),
     ({"H": 1 << 31}, -1, "sizes"),
-    ({"T": 1 << 24}, -2, "rows"),
+    ({"T": 1 << 31}, -1, "sizes"),
+    ({"T": 1 << 23, "H": 16385}, -2, "one launch"),
     ({"x": 1, "y": 0}, -1, "x's type"),
     ({"x": 1, "y": 2}, -1, "x's type"),
     ({"x": 5}, -1, "dtype"),
@@ -105,7 +106,9 @@ def test_layernorm_backward_refusals(lib):
         return lib.pmoe_layernorm_backward(FAKE, g, FAKE, x, None, 0, mean, FAKE, T, H, FAKE, FAKE, FAKE, ws, nbytes,
                                            None)
 
-    assert bwd(g=0, x=1) == -1 and bwd(T=1 << 24) == -2
+    assert bwd(g=0, x=1) == -1 and bwd(T=1 << 23, H=20000) == -2
+    assert lib.pmoe_layernorm_backward_workspace_size(0, 8) == 0
+    assert lib.pmoe_layernorm_backward_workspace_size(1000, 2048) >= 2 * 125 * 2048 * 4
     assert bwd(mean=None) == -1 and "null tensor" in message(lib)
     assert bwd(nbytes=0) == -3 and bwd(ws=None) == -3
     assert bwd(ws=ctypes.c_void_p(260)) == -1 and "aligned" in message(lib)
