@@ -18,32 +18,32 @@ from ._lib import require_gpu
 from .moe import _empty_like_none, _refuse_capture, _stage
 
 
-def _backward(grad, x, weight, bias, mean, rstd, needs):
+def _backward(grad, x, weight, bias, stats, needs):
     """The gradients of x, weight and bias (None where ``needs`` says so)."""
     _refuse_capture("layer_norm_bwd")
     dt = next((p.dtype for p in (weight, bias) if p is not None), torch.float32)
     with _stage("layernorm_bwd"):
-        return ops.layernorm_backward(grad, x, weight, mean, rstd, dt, *needs)
+        return ops.layernorm_backward(grad, x, weight, stats, dt, *needs)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype):
         with _stage("layernorm"):
-            out, mean, rstd = ops.layernorm_forward(x, weight, bias, eps, out_dtype)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+            out, stats = ops.layernorm_forward(x, weight, bias, eps, out_dtype)
+        ctx.save_for_backward(x, weight, bias, stats)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        return (*_backward(grad.contiguous(), x, weight, bias, mean, rstd, ctx.needs_input_grad[:3]), None, None)
+        x, weight, bias, stats = ctx.saved_tensors
+        return (*_backward(grad.contiguous(), x.contiguous(), weight, bias, stats, ctx.needs_input_grad[:3]), None, None)
 
 
 @torch.library.custom_op("pmoe::layer_norm_fwd", mutates_args=(),
                          schema="(Tensor x, Tensor? weight, Tensor? bias, float eps, ScalarType out_dtype) -> "
-                                "(Tensor, Tensor, Tensor)")
+                                "(Tensor, Tensor)")
 def _layer_norm_fwd(x, weight, bias, eps, out_dtype):
     with _stage("layernorm"):
         return ops.layernorm_forward(x, weight, bias, eps, out_dtype)
@@ -51,37 +51,36 @@ def _layer_norm_fwd(x, weight, bias, eps, out_dtype):
 
 @_layer_norm_fwd.register_fake
 def _(x, weight, bias, eps, out_dtype):
-    f32 = torch.float32
-    return torch.empty_like(x, dtype=out_dtype), x.new_empty(x.shape[0], dtype=f32), x.new_empty(x.shape[0], dtype=f32)
+    return torch.empty_like(x, dtype=out_dtype), x.new_empty(2, x.numel() // x.shape[-1], dtype=torch.float32)
 
 
 @torch.library.custom_op("pmoe::layer_norm_bwd", mutates_args=(),
-                         schema="(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor mean, Tensor rstd, "
-                                "bool[] needs) -> (Tensor, Tensor, Tensor)")
-def _layer_norm_bwd(grad, x, weight, bias, mean, rstd, needs):
-    got = _backward(grad, x, weight, bias, mean, rstd, needs)
+                         schema="(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor stats, bool[] needs) -> "
+                                "(Tensor, Tensor, Tensor)")
+def _layer_norm_bwd(grad, x, weight, bias, stats, needs):
+    got = _backward(grad, x, weight, bias, stats, needs)
     return tuple(g if g is not None else _empty_like_none(x) for g in got)
 
 
 @_layer_norm_bwd.register_fake
-def _(grad, x, weight, bias, mean, rstd, needs):
+def _(grad, x, weight, bias, stats, needs):
     return tuple(torch.empty_like(t) if need else _empty_like_none(x) for need, t in zip(needs, (x, weight, bias)))
 
 
 def _setup(ctx, inputs, output):
     x, weight, bias, _eps, _out_dtype = inputs
-    _out, mean, rstd = output
-    ctx.save_for_backward(x, weight, bias, mean, rstd)
-    ctx.mark_non_differentiable(mean, rstd)
+    _out, stats = output
+    ctx.save_for_backward(x, weight, bias, stats)
+    ctx.mark_non_differentiable(stats)
     ctx.set_materialize_grads(False)
 
 
-def _autograd(ctx, grad, _gm, _gr):
+def _autograd(ctx, grad, _gs):
     if grad is None:
         return (None,) * 5
-    x, weight, bias, mean, rstd = ctx.saved_tensors
+    x, weight, bias, stats = ctx.saved_tensors
     needs = [bool(n) for n in ctx.needs_input_grad[:3]]
-    got = torch.ops.pmoe.layer_norm_bwd(grad.contiguous(), x, weight, bias, mean, rstd, needs)
+    got = torch.ops.pmoe.layer_norm_bwd(grad.contiguous(), x, weight, bias, stats, needs)
     return (*(g if need else None for g, need in zip(got, needs)), None, None)
 
 
@@ -110,13 +109,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         f"layer_norm: {out_dtype} from {x.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         weight, bias = weight.float(), bias.float()
-    rows = x.reshape(-1, H).contiguous()
-    weight, bias = (p if p is None else p.contiguous() for p in (weight, bias))
+    x, weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (x, weight, bias))
     if torch.compiler.is_compiling():
-        out = torch.ops.pmoe.layer_norm_fwd(rows, weight, bias, float(eps), out_dtype)[0]
-    elif torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rows, weight, bias)):
-        out = _LayerNorm.apply(rows, weight, bias, float(eps), out_dtype)
-    else:
-        with _stage("layernorm"):
-            out = ops.layernorm_forward(rows, weight, bias, float(eps), out_dtype, stats=False)[0]
-    return out.reshape(x.shape)
+        return torch.ops.pmoe.layer_norm_fwd(x, weight, bias, float(eps), out_dtype)[0]
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in (x, weight, bias)]):
+        return _LayerNorm.apply(x, weight, bias, float(eps), out_dtype)
+    with _stage("layernorm"):
+        return ops.layernorm_forward(x, weight, bias, float(eps), out_dtype, stats=False)[0]

@@ -350,39 +350,44 @@ def dispatch_rmsnorm_backward(grad_x_perm, inv_pos, grad_normed_add, x, weight, 
 
 
 def layernorm_forward(x, weight, bias, eps: float, out_dtype, stats: bool = True):
-    """torch.nn.LayerNorm over the rows of x (T,H) in fp32 arithmetic -> out (T,H) out_dtype, mean and
-    rstd (T,) fp32 (None without ``stats``). weight and bias (H,), one dtype, or None."""
+    """torch.nn.LayerNorm over the last dimension of x (..., H) in fp32 arithmetic -> out (..., H) out_dtype
+    and stats (2, T) fp32, the T rows' means and reciprocal deviations (None without ``stats``). weight and
+    bias (H,), one dtype, or None."""
     require_gpu(x, weight, bias)
-    T, H = x.shape
+    H = x.shape[-1]
+    T = x.numel() // H
     assert x.is_contiguous() and all(p is None or (p.is_contiguous() and p.shape == (H,) and p.device == x.device)
                                      for p in (weight, bias))
     assert weight is None or bias is None or weight.dtype == bias.dtype
     wdt = next((p.dtype for p in (weight, bias) if p is not None), torch.float32)
-    out = torch.empty(T, H, dtype=out_dtype, device=x.device)
-    mean, rstd = (torch.empty(T, dtype=torch.float32, device=x.device) if stats else None for _ in range(2))
+    out = torch.empty_like(x, dtype=out_dtype)
+    kept = torch.empty(2, T, dtype=torch.float32, device=x.device) if stats else None
+    mean = ptr(kept) if stats else None
     with on_device(x):
         call("pmoe_layernorm_forward", ptr(x), dtype_code(x.dtype), ptr(weight), ptr(bias), dtype_code(wdt),
-             float(eps), T, H, ptr(out), dtype_code(out_dtype), ptr(mean), ptr(rstd), stream_of(x))
-    return out, mean, rstd
+             float(eps), T, H, ptr(out), dtype_code(out_dtype), mean, mean + 4 * T if stats else None, stream_of(x))
+    return out, kept
 
 
-def layernorm_backward(grad, x, weight, mean, rstd, weight_dtype=torch.float32, need_x: bool = True,
+def layernorm_backward(grad, x, weight, stats, weight_dtype=torch.float32, need_x: bool = True,
                        need_weight: bool = True, need_bias: bool = True):
     """-> grad_x (x.dtype), grad_weight and grad_bias (weight_dtype, ``weight``'s own when it is given);
-    None where not needed. grad has the forward's out_dtype."""
-    require_gpu(grad, x, weight, mean, rstd)
-    T, H = x.shape
+    None where not needed. stats: the forward's; grad has its out_dtype."""
+    require_gpu(grad, x, weight, stats)
+    H = x.shape[-1]
+    T = x.numel() // H
     assert grad.shape == x.shape and grad.is_contiguous() and x.is_contiguous()
     assert weight is None or (weight.dtype == weight_dtype and weight.shape == (H,) and weight.is_contiguous())
-    assert mean.shape == rstd.shape == (T,) and mean.dtype == rstd.dtype == torch.float32
+    assert stats.shape == (2, T) and stats.dtype == torch.float32 and stats.is_contiguous()
     dev = x.device
     gx = torch.empty_like(x) if need_x else None
     gw = torch.empty(H, dtype=weight_dtype, device=dev) if need_weight else None
     gb = torch.empty(H, dtype=weight_dtype, device=dev) if need_bias else None
     ws = workspace(size("pmoe_layernorm_backward_workspace_size", T, H) if need_weight or need_bias else 0, dev)
+    mean = ptr(stats)
     with on_device(x):
         call("pmoe_layernorm_backward", ptr(grad), dtype_code(grad.dtype), ptr(x), dtype_code(x.dtype), ptr(weight),
-             dtype_code(weight_dtype), ptr(mean), ptr(rstd), T, H, ptr(gx), ptr(gw), ptr(gb), ptr(ws), ws.numel(),
+             dtype_code(weight_dtype), mean, mean + 4 * T, T, H, ptr(gx), ptr(gw), ptr(gb), ptr(ws), ws.numel(),
              stream_of(x))
     return gx, gw, gb
 

@@ -186,5 +186,5 @@ def test_fake_shapes_of_the_checkpointed_ops():
         assert out[6].shape == (T * K, 2, 2) and out[6].dtype == torch.uint8
         plain = torch.ops.pmoe.expert_ffn_fwd(hid, idx, w, gu, dn)
         assert plain[5].dtype == torch.bfloat16 and plain[6].shape == (T * K, I)
-        y, mean, rstd = torch.ops.pmoe.layer_norm_fwd(torch.empty(5, 8), None, None, 1e-5, torch.float16)
-        assert y.dtype == torch.float16 and mean.shape == rstd.shape == (5,)
+        y, stats = torch.ops.pmoe.layer_norm_fwd(torch.empty(3, 5, 8), None, None, 1e-5, torch.float16)
+        assert y.shape == (3, 5, 8) and y.dtype == torch.float16 and stats.shape == (2, 15)
