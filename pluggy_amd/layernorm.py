@@ -21,9 +21,9 @@ from .moe import _empty_like_none, _refuse_capture, _stage
 def _backward(grad, x, weight, bias, stats, needs):
     """The gradients of x, weight and bias (None where ``needs`` says so)."""
     _refuse_capture("layer_norm_bwd")
-    dt = next((p.dtype for p in (weight, bias) if p is not None), torch.float32)
+    dt = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
     with _stage("layernorm_bwd"):
-        return ops.layernorm_backward(grad, x, weight, stats, dt, *needs)
+        return ops._layernorm_backward(grad, x, weight, stats, dt, *needs)
 
 
 class _LayerNorm(torch.autograd.Function):

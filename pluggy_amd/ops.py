@@ -375,20 +375,27 @@ def layernorm_backward(grad, x, weight, stats, weight_dtype=torch.float32, need_
     None where not needed. stats: the forward's; grad has its out_dtype."""
     require_gpu(grad, x, weight, stats)
     H = x.shape[-1]
-    T = x.numel() // H
     assert grad.shape == x.shape and grad.is_contiguous() and x.is_contiguous()
     assert weight is None or (weight.dtype == weight_dtype and weight.shape == (H,) and weight.is_contiguous())
-    assert stats.shape == (2, T) and stats.dtype == torch.float32 and stats.is_contiguous()
-    dev = x.device
+    assert stats.shape == (2, x.numel() // H) and stats.dtype == torch.float32 and stats.is_contiguous()
+    return _layernorm_backward(grad, x, weight, stats, weight_dtype, need_x, need_weight, need_bias)
+
+
+def _layernorm_backward(grad, x, weight, stats, weight_dtype, need_x, need_weight, need_bias):
+    """``layernorm_backward`` on what the forward kept (autograd's thread: every microsecond here is waited for)."""
+    H, T, dev = x.shape[-1], stats.shape[1], x.device
     gx = torch.empty_like(x) if need_x else None
     gw = torch.empty(H, dtype=weight_dtype, device=dev) if need_weight else None
     gb = torch.empty(H, dtype=weight_dtype, device=dev) if need_bias else None
-    ws = workspace(size("pmoe_layernorm_backward_workspace_size", T, H) if need_weight or need_bias else 0, dev)
-    mean = ptr(stats)
+    ws, nbytes = None, 0
+    if need_weight or need_bias:
+        nbytes = size("pmoe_layernorm_backward_workspace_size", T, H)
+        ws = workspace(nbytes, dev)
+    mean = stats.data_ptr()
     with on_device(x):
-        call("pmoe_layernorm_backward", ptr(grad), dtype_code(grad.dtype), ptr(x), dtype_code(x.dtype), ptr(weight),
-             dtype_code(weight_dtype), mean, mean + 4 * T, T, H, ptr(gx), ptr(gw), ptr(gb), ptr(ws), ws.numel(),
-             stream_of(x))
+        call("pmoe_layernorm_backward", grad.data_ptr(), dtype_code(grad.dtype), x.data_ptr(), dtype_code(x.dtype),
+             ptr(weight), dtype_code(weight_dtype), mean, mean + 4 * T, T, H, ptr(gx), ptr(gw), ptr(gb), ptr(ws),
+             nbytes, stream_of(x))
     return gx, gw, gb
 
 
