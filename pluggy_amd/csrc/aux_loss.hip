@@ -281,7 +281,7 @@ __global__ __launch_bounds__(stats_block(LPR * V)) void aux_stats_kernel(AuxLaye
       mx = v[0];
 #pragma unroll
       for (int i = 1; i < V; ++i) mx = fmaxf(mx, v[i]);
-      mx = row_fmax<LPR>(mx);
+      mx = row_fmax<LPR>(mx) + 0.0f;  // never -0: +0 and -0 both have the key 0 then
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float d = mx - v[i];

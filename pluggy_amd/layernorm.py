@@ -21,6 +21,7 @@ from .moe import _empty_like_none, _refuse_capture, _stage
 def _backward(grad, x, weight, bias, stats, needs):
     """The gradients of x, weight and bias (None where ``needs`` says so)."""
     _refuse_capture("layer_norm_bwd")
+    require_gpu(x, weight, stats)  # a saved-tensor hook may give host tensors back
     dt = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
     with _stage("layernorm_bwd"):
         return ops._layernorm_backward(grad, x, weight, stats, dt, *needs)

@@ -430,23 +430,29 @@ class _Layers:
         self.rows = [s[0] for s in shapes]
         self.L, self.E, self.dtype, self.device = len(logits), E, first.dtype, first.device
         self.row_array = (ctypes.c_int64 * self.L)(*self.rows)
+        self.pointers = _pointers(logits)
         self.tail = (self.row_array, self.L, dtype_code(first.dtype), ptr(mask), mask_rows, E)
+
+    def hold(self, logits, mask):
+        """Whether these are the tensors that were checked, as they lay then."""
+        return (bytes(self.pointers) == bytes(_pointers(logits)) and self.tail[3] == ptr(mask)
+                and all([t.is_contiguous() for t in logits]))
 
 
 def aux_loss_forward(logits, top_k: int, aux_coef: float, z_coef: float, mask=None):
     """The layers' logits, a list of (N_i, E) -> loss, load balance and z-loss (() fp32), expert_counts
     (L, E) int32, coef (E + 1,) fp32 for ``aux_loss_backward``. mask (N,) bool or uint8: rows that count."""
-    return _aux_loss_forward(_Layers(logits, mask), logits, top_k, aux_coef, z_coef)
+    return _aux_loss_forward(_Layers(logits, mask), top_k, aux_coef, z_coef)
 
 
-def _aux_loss_forward(layers, logits, top_k, aux_coef, z_coef):
+def _aux_loss_forward(layers, top_k, aux_coef, z_coef):
     dev, L, E = layers.device, layers.L, layers.E
     losses = [torch.empty((), dtype=torch.float32, device=dev) for _ in range(3)]
     counts = torch.empty(L, E, dtype=torch.int32, device=dev)
     coef = torch.empty(E + 1, dtype=torch.float32, device=dev)
     ws = workspace(size("pmoe_aux_loss_forward_workspace_size", layers.row_array, L, E), dev)
     with on_device(coef):
-        call("pmoe_aux_loss_forward", _pointers(logits), *layers.tail, top_k, aux_coef, z_coef, *map(ptr, losses),
+        call("pmoe_aux_loss_forward", layers.pointers, *layers.tail, top_k, aux_coef, z_coef, *map(ptr, losses),
              ptr(counts), ptr(coef), ptr(ws), ws.numel(), stream_of(coef))
     return (*losses, counts, coef)
 
@@ -472,10 +478,10 @@ def aux_loss_from_stats(counts, prob_sums, lse_sq_sums, n: int, top_k: int, aux_
 def aux_loss_backward(logits, coef, grad_loss, aux_coef: float, z_coef: float, mask=None, needs=None):
     """-> every layer's gradient (N_i, E) in its logits' dtype (None where needs[i] is false); grad_loss:
     the loss's gradient, one fp32 value on the device."""
-    return _aux_loss_backward(_Layers(logits, mask), logits, coef, grad_loss, aux_coef, z_coef, needs)
+    return _aux_loss_backward(_Layers(logits, mask), coef, grad_loss, aux_coef, z_coef, needs)
 
 
-def _aux_loss_backward(layers, logits, coef, grad_loss, aux_coef, z_coef, needs=None):
+def _aux_loss_backward(layers, coef, grad_loss, aux_coef, z_coef, needs=None):
     require_gpu(coef, grad_loss)
     E = layers.E
     assert grad_loss.numel() == 1 and grad_loss.dtype == torch.float32 and coef.shape == (E + 1,)
@@ -488,7 +494,7 @@ def _aux_loss_backward(layers, logits, coef, grad_loss, aux_coef, z_coef, needs=
     if sizes is not layers.rows:
         grads = [g if k else None for g, k in zip(grads, needs)]
     with on_device(coef):
-        call("pmoe_aux_loss_backward", _pointers(logits), _pointers(grads), *layers.tail, ptr(coef), ptr(grad_loss),
+        call("pmoe_aux_loss_backward", layers.pointers, _pointers(grads), *layers.tail, ptr(coef), ptr(grad_loss),
              aux_coef, z_coef, stream_of(coef))
     return grads
 

@@ -147,7 +147,7 @@ class _RouterAuxLoss(torch.autograd.Function):
     def forward(ctx, layers, top_k, aux_coef, z_coef, mask, stats, *logits):
         with _stage("aux_loss"):
             if stats is None:
-                *losses, counts, coef = ops._aux_loss_forward(layers, logits, top_k, aux_coef, z_coef)
+                *losses, counts, coef = ops._aux_loss_forward(layers, top_k, aux_coef, z_coef)
             else:
                 *losses, counts, coef = ops.aux_loss_from_stats(
                     [s.expert_counts for s in stats], [s.prob_sum for s in stats], [s.lse_sq_sum for s in stats],
@@ -167,13 +167,12 @@ class _RouterAuxLoss(torch.autograd.Function):
         if g_loss is None or not any(needs):
             return (None,) * (6 + len(logits))
         _refuse_capture("aux_loss_bwd")
-        # a saved-tensor hook may have given other tensors back: checked again unless they lie where they lay
         layers = ctx.layers
-        if layers.tail[3] != ops.ptr(mask) or not all([t.is_contiguous() for t in logits]):
+        if not layers.hold(logits, mask):  # a saved-tensor hook gave others back
             logits = [t.contiguous() for t in logits]
             layers = ops._Layers(logits, mask)
         with _stage("aux_loss_bwd"):
-            grads = ops._aux_loss_backward(layers, logits, coef, g_loss.float().contiguous(), *ctx.coefs, needs)
+            grads = ops._aux_loss_backward(layers, coef, g_loss.float().contiguous(), *ctx.coefs, needs)
         return (None, None, None, None, None, None, *grads)
 
 

@@ -413,3 +413,28 @@ def test_backward_under_capture_raises(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="not supported under HIP graph capture"):
         r.loss.backward()
+
+
+def test_host_tensors_from_a_hook_are_refused():
+    """A hook that moves the saved logits to the host and forgets to bring them back."""
+    import pluggy_amd
+
+    logits = draw(2, 20, 8, "fp32", 24)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t if t.dim() == 2 else t.to(DEV)):
+        r = pluggy_amd.router_aux_loss(logits, 8, 2)
+    with pytest.raises(RuntimeError, match="ROCm GPU tensors only"):
+        r.loss.backward()
+
+
+@pytest.mark.parametrize("E,K", [(4, 1), (20, 3), (128, 4)])
+def test_zeros_of_both_signs_at_the_top(E, K):
+    """The largest logits are zeros of both signs, in either order, above others: equal, so the lower ids."""
+    g = gen(25 + E)
+    l = -1.0 - torch.rand(64, E, generator=g)
+    for t in range(64):
+        at = torch.randperm(E, generator=g)[:K + 1]
+        l[t, at] = torch.where(torch.rand(K + 1, generator=g) < 0.5, 0.0, -0.0)
+    logits = [l.to(DEV).requires_grad_()]
+    r, grads = run(logits, K, 1.0, 0.1)
+    ref = reference([torch.where(l == 0, 0.0, l)], K, 1.0, 0.1)
+    check(r, grads, ref, 1.0, 0.1)

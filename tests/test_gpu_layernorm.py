@@ -320,3 +320,13 @@ def test_moe_sublayer_with_a_layer_norm(amp):
     g = torch.randn_like(y)
     for a, c in zip(torch.autograd.grad(y, params, g), torch.autograd.grad(want, params, g)):
         assert torch.equal(a, c) and a.abs().sum() > 0
+
+
+def test_host_tensors_from_a_hook_are_refused():
+    import pluggy_amd
+
+    x, w, b, g = inputs(8, 64, torch.float32, torch.float32, 26)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t):
+        y = pluggy_amd.layer_norm(x.requires_grad_(), w, b)
+    with pytest.raises(RuntimeError, match="ROCm GPU tensors only"):
+        torch.autograd.grad(y, [x], g)
