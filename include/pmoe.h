@@ -451,6 +451,10 @@ enum {
 PMOE_API int pmoe_expert_gemm_tile_rows(int kind, int64_t P, int64_t E, int64_t H, int64_t I, int dtype,
                                         int num_cus);
 
+/* Whether a HIP graph is being captured on the stream: 1 or 0. The backward
+ * passes refuse to run then. Launches nothing. */
+PMOE_API int pmoe_stream_capturing(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

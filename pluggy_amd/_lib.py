@@ -81,6 +81,7 @@ SIGNATURES = {
     "pmoe_expert_ffn_forward_noalloc": (_INT, [_P, _P, _P, _INT, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P,
                                                _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "pmoe_expert_ffn_backward_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _INT]),
+    "pmoe_stream_capturing": (_INT, [_P]),
     "pmoe_expert_gemm_tile_rows": (_INT, [_INT, _I64, _I64, _I64, _I64, _INT, _INT]),
     "pmoe_expert_ffn_backward": (_INT, [_P, _P, _INT, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P,
                                         _P, _P, _P, _P, _P, _P, _INT, _P, _SZ, _P]),
@@ -88,6 +89,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_nodes = None
 
 
 def load() -> ctypes.CDLL:
@@ -107,6 +109,20 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def nodes():
+    """The C++ autograd nodes (``_autograd.so``, built from ``csrc/autograd.cpp`` over ``libpmoe.so``)."""
+    global _nodes
+    if _nodes is None:
+        load()
+        try:
+            from . import _autograd
+        except ImportError as e:
+            raise RuntimeError(f"pmoe autograd nodes not loaded ({e}); build them for this torch with "
+                               "`python -m pluggy_amd.build`") from e
+        _nodes = _autograd
+    return _nodes
 
 
 def call(name: str, *args) -> None:

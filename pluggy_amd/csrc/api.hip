@@ -826,6 +826,11 @@ PMOE_API int pmoe_expert_ffn_backward(const void* grad_out, const void* hidden, 
 
 // ------------------------------------------------------- engine queries
 
+PMOE_API int pmoe_stream_capturing(void* stream) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(as_stream(stream), &st) == hipSuccess && st != hipStreamCaptureStatusNone ? 1 : 0;
+}
+
 PMOE_API int pmoe_expert_gemm_tile_rows(int kind, int64_t P, int64_t E, int64_t H, int64_t I, int dtype,
                                         int num_cus) {
   PMOE_REQUIRE(kind >= EG_GATE_UP_FWD && kind <= EG_GATE_UP_WGRAD, "expert_gemm_tile_rows: unknown kind %d", kind);

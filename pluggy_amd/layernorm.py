@@ -2,8 +2,8 @@
 
 ``layer_norm`` is ``torch.nn.functional.layer_norm`` over the last dimension,
 forward and backward, in fp32 arithmetic; ``moe_sublayer`` calls it for a block
-whose norm is a ``torch.nn.LayerNorm``. Eager calls go through one
-``torch.autograd.Function`` (or, where no gradient is wanted, straight to the
+whose norm is a ``torch.nn.LayerNorm``. Eager calls go through one autograd node
+in C++ (``csrc/autograd.cpp``; where no gradient is wanted, straight to the
 kernel); under ``torch.compile`` they are the custom ops ``pmoe::layer_norm_fwd``
 and ``pmoe::layer_norm_bwd``, which trace without graph breaks.
 """
@@ -11,35 +11,10 @@ and ``pmoe::layer_norm_bwd``, which trace without graph breaks.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
-from ._lib import require_gpu
+from ._lib import nodes, on_device, require_gpu, stream_of
 from .moe import _empty_like_none, _refuse_capture, _stage
-
-
-def _backward(grad, x, weight, bias, stats, needs):
-    """The gradients of x, weight and bias (None where ``needs`` says so)."""
-    _refuse_capture("layer_norm_bwd")
-    require_gpu(x, weight, stats)  # a saved-tensor hook may give host tensors back
-    dt = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-    with _stage("layernorm_bwd"):
-        return ops._layernorm_backward(grad, x, weight, stats, dt, *needs)
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, out_dtype):
-        with _stage("layernorm"):
-            out, stats = ops.layernorm_forward(x, weight, bias, eps, out_dtype)
-        ctx.save_for_backward(x, weight, bias, stats)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        x, weight, bias, stats = ctx.saved_tensors
-        return (*_backward(grad.contiguous(), x.contiguous(), weight, bias, stats, ctx.needs_input_grad[:3]), None, None)
 
 
 @torch.library.custom_op("pmoe::layer_norm_fwd", mutates_args=(),
@@ -59,7 +34,10 @@ def _(x, weight, bias, eps, out_dtype):
                          schema="(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor stats, bool[] needs) -> "
                                 "(Tensor, Tensor, Tensor)")
 def _layer_norm_bwd(grad, x, weight, bias, stats, needs):
-    got = _backward(grad, x, weight, bias, stats, needs)
+    _refuse_capture("layer_norm_bwd")
+    dt = next((p.dtype for p in (weight, bias) if p is not None), torch.float32)
+    with _stage("layernorm_bwd"):
+        got = ops.layernorm_backward(grad, x, weight, stats, dt, *needs)
     return tuple(g if g is not None else _empty_like_none(x) for g in got)
 
 
@@ -114,6 +92,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if torch.compiler.is_compiling():
         return torch.ops.pmoe.layer_norm_fwd(x, weight, bias, float(eps), out_dtype)[0]
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in (x, weight, bias)]):
-        return _LayerNorm.apply(x, weight, bias, float(eps), out_dtype)
+        with _stage("layernorm"), on_device(x):
+            return nodes().layer_norm(x, weight, bias, float(eps), out_dtype, stream_of(x))
     with _stage("layernorm"):
         return ops.layernorm_forward(x, weight, bias, float(eps), out_dtype, stats=False)[0]

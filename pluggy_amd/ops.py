@@ -7,7 +7,6 @@ freshly allocated on the input's device and stream.
 
 from __future__ import annotations
 
-import ctypes
 
 import torch
 
@@ -378,12 +377,7 @@ def layernorm_backward(grad, x, weight, stats, weight_dtype=torch.float32, need_
     assert grad.shape == x.shape and grad.is_contiguous() and x.is_contiguous()
     assert weight is None or (weight.dtype == weight_dtype and weight.shape == (H,) and weight.is_contiguous())
     assert stats.shape == (2, x.numel() // H) and stats.dtype == torch.float32 and stats.is_contiguous()
-    return _layernorm_backward(grad, x, weight, stats, weight_dtype, need_x, need_weight, need_bias)
-
-
-def _layernorm_backward(grad, x, weight, stats, weight_dtype, need_x, need_weight, need_bias):
-    """``layernorm_backward`` on what the forward kept (autograd's thread: every microsecond here is waited for)."""
-    H, T, dev = x.shape[-1], stats.shape[1], x.device
+    T, dev = stats.shape[1], x.device
     gx = torch.empty_like(x) if need_x else None
     gw = torch.empty(H, dtype=weight_dtype, device=dev) if need_weight else None
     gb = torch.empty(H, dtype=weight_dtype, device=dev) if need_bias else None
@@ -397,106 +391,6 @@ def _layernorm_backward(grad, x, weight, stats, weight_dtype, need_x, need_weigh
              ptr(weight), dtype_code(weight_dtype), mean, mean + 4 * T, T, H, ptr(gx), ptr(gw), ptr(gb), ptr(ws),
              nbytes, stream_of(x))
     return gx, gw, gb
-
-
-# ------------------------------------------------------ router auxiliary loss
-
-
-def _pointers(tensors):
-    """A host array of the tensors' device pointers (None: a null one)."""
-    return (ctypes.c_void_p * len(tensors))(*[0 if t is None else t.data_ptr() for t in tensors])
-
-
-class _Layers:
-    """The layers' logits as the entry points take them: one dtype, device and number of experts, contiguous."""
-
-    def __init__(self, logits, mask):
-        first = logits[0]
-        shapes = [t.shape for t in logits]
-        E = shapes[0][-1]
-        assert all([len(s) == 2 and s[1] == E for s in shapes]), f"logits (N, E) of one E, got {shapes}"
-        assert len({t.dtype for t in logits}) == 1, f"logits of one type, got {[t.dtype for t in logits]}"
-        devices = {t.get_device() for t in logits}  # -1: not on a GPU
-        if devices != {first.get_device()} or -1 in devices:
-            require_gpu(*logits)
-            raise AssertionError(f"logits on one device, got {devices}")
-        assert all([t.is_contiguous() for t in logits])
-        mask_rows = 0
-        if mask is not None:
-            require_gpu(mask)
-            assert mask.dtype in (torch.bool, torch.uint8) and mask.dim() == 1 and mask.is_contiguous()
-            assert mask.device == first.device
-            mask_rows = mask.shape[0]
-        self.rows = [s[0] for s in shapes]
-        self.L, self.E, self.dtype, self.device = len(logits), E, first.dtype, first.device
-        self.row_array = (ctypes.c_int64 * self.L)(*self.rows)
-        self.pointers = _pointers(logits)
-        self.tail = (self.row_array, self.L, dtype_code(first.dtype), ptr(mask), mask_rows, E)
-
-    def hold(self, logits, mask):
-        """Whether these are the tensors that were checked, as they lay then."""
-        return (bytes(self.pointers) == bytes(_pointers(logits)) and self.tail[3] == ptr(mask)
-                and all([t.is_contiguous() for t in logits]))
-
-
-def aux_loss_forward(logits, top_k: int, aux_coef: float, z_coef: float, mask=None):
-    """The layers' logits, a list of (N_i, E) -> loss, load balance and z-loss (() fp32), expert_counts
-    (L, E) int32, coef (E + 1,) fp32 for ``aux_loss_backward``. mask (N,) bool or uint8: rows that count."""
-    return _aux_loss_forward(_Layers(logits, mask), top_k, aux_coef, z_coef)
-
-
-def _aux_loss_forward(layers, top_k, aux_coef, z_coef):
-    dev, L, E = layers.device, layers.L, layers.E
-    losses = [torch.empty((), dtype=torch.float32, device=dev) for _ in range(3)]
-    counts = torch.empty(L, E, dtype=torch.int32, device=dev)
-    coef = torch.empty(E + 1, dtype=torch.float32, device=dev)
-    ws = workspace(size("pmoe_aux_loss_forward_workspace_size", layers.row_array, L, E), dev)
-    with on_device(coef):
-        call("pmoe_aux_loss_forward", layers.pointers, *layers.tail, top_k, aux_coef, z_coef, *map(ptr, losses),
-             ptr(counts), ptr(coef), ptr(ws), ws.numel(), stream_of(coef))
-    return (*losses, counts, coef)
-
-
-def aux_loss_from_stats(counts, prob_sums, lse_sq_sums, n: int, top_k: int, aux_coef: float, z_coef: float):
-    """``aux_loss_forward`` from the routers' statistics (lists, one entry a layer) of n rows in all."""
-    require_gpu(*counts, *prob_sums, *lse_sq_sums)
-    L, E, dev = len(counts), counts[0].shape[0], counts[0].device
-    for ts, shape, dt in ((counts, (E,), torch.int32), (prob_sums, (E,), torch.float32),
-                          (lse_sq_sums, (1,), torch.float32)):
-        assert len(ts) == L and all(t.shape == shape and t.dtype == dt and t.is_contiguous() and t.device == dev
-                                    for t in ts)
-    losses = tuple(torch.empty((), dtype=torch.float32, device=dev) for _ in range(3))
-    out = torch.empty(L, E, dtype=torch.int32, device=dev)
-    coef = torch.empty(E + 1, dtype=torch.float32, device=dev)
-    ws = workspace(size("pmoe_aux_loss_from_stats_workspace_size", L, E), dev)
-    with on_device(coef):
-        call("pmoe_aux_loss_from_stats", _pointers(counts), _pointers(prob_sums), _pointers(lse_sq_sums), L, n, E,
-             top_k, aux_coef, z_coef, *map(ptr, losses), ptr(out), ptr(coef), ptr(ws), ws.numel(), stream_of(coef))
-    return (*losses, out, coef)
-
-
-def aux_loss_backward(logits, coef, grad_loss, aux_coef: float, z_coef: float, mask=None, needs=None):
-    """-> every layer's gradient (N_i, E) in its logits' dtype (None where needs[i] is false); grad_loss:
-    the loss's gradient, one fp32 value on the device."""
-    return _aux_loss_backward(_Layers(logits, mask), coef, grad_loss, aux_coef, z_coef, needs)
-
-
-def _aux_loss_backward(layers, coef, grad_loss, aux_coef, z_coef, needs=None):
-    require_gpu(coef, grad_loss)
-    E = layers.E
-    assert grad_loss.numel() == 1 and grad_loss.dtype == torch.float32 and coef.shape == (E + 1,)
-    # one allocation for all layers; each gradient is its rows
-    if needs is None or all(needs):
-        sizes = layers.rows
-    else:
-        sizes = [n if k else 0 for n, k in zip(layers.rows, needs)]
-    grads = torch.empty(sum(sizes), E, dtype=layers.dtype, device=layers.device).split(sizes)
-    if sizes is not layers.rows:
-        grads = [g if k else None for g, k in zip(grads, needs)]
-    with on_device(coef):
-        call("pmoe_aux_loss_backward", layers.pointers, _pointers(grads), *layers.tail, ptr(coef), ptr(grad_loss),
-             aux_coef, z_coef, stream_of(coef))
-    return grads
 
 
 # ------------------------------------------ activation checkpoints in 8 bits

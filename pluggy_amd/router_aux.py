@@ -33,11 +33,9 @@ from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
-from . import ops
-from ._lib import require_gpu
-from .moe import RouterStats, _refuse_capture, _stage
+from ._lib import nodes, on_device, require_gpu, stream_of
+from .moe import RouterStats, _stage
 
 
 def _totals(stats: list[RouterStats]) -> tuple[int, torch.Tensor, torch.Tensor]:
@@ -142,38 +140,26 @@ class RouterAuxLoss:
     expert_counts: torch.Tensor  # (L, E) int32: valid rows that picked each expert, by layer
 
 
-class _RouterAuxLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, layers, top_k, aux_coef, z_coef, mask, stats, *logits):
-        with _stage("aux_loss"):
-            if stats is None:
-                *losses, counts, coef = ops._aux_loss_forward(layers, top_k, aux_coef, z_coef)
-            else:
-                *losses, counts, coef = ops.aux_loss_from_stats(
-                    [s.expert_counts for s in stats], [s.prob_sum for s in stats], [s.lse_sq_sum for s in stats],
-                    sum(int(s.tokens) for s in stats), top_k, aux_coef, z_coef)
-        ctx.save_for_backward(coef, mask, *logits)
-        ctx.layers, ctx.coefs = layers, (aux_coef, z_coef)
-        loss, balance, z = losses
-        ctx.mark_non_differentiable(balance, z, counts)
-        ctx.set_materialize_grads(False)
-        return loss, balance, z, counts
+def _check_layers(logits, mask):
+    """One dtype, device and number of experts, contiguous: what the kernels read."""
+    shapes = [t.shape for t in logits]
+    E = shapes[0][-1]
+    assert all([len(s) == 2 and s[1] == E for s in shapes]), f"logits (N, E) of one E, got {shapes}"
+    assert len({t.dtype for t in logits}) == 1, f"logits of one type, got {[t.dtype for t in logits]}"
+    devices = {t.get_device() for t in logits}  # -1: not on a GPU
+    if len(devices) != 1 or -1 in devices:
+        require_gpu(*logits)
+        raise AssertionError(f"logits on one device, got {devices}")
+    assert mask is None or mask.device == logits[0].device, f"token_mask on {mask.device}"
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_loss, _gb, _gz, _gc):
-        coef, mask, *logits = ctx.saved_tensors
-        needs = ctx.needs_input_grad[6:]
-        if g_loss is None or not any(needs):
-            return (None,) * (6 + len(logits))
-        _refuse_capture("aux_loss_bwd")
-        layers = ctx.layers
-        if not layers.hold(logits, mask):  # a saved-tensor hook gave others back
-            logits = [t.contiguous() for t in logits]
-            layers = ops._Layers(logits, mask)
-        with _stage("aux_loss_bwd"):
-            grads = ops._aux_loss_backward(layers, coef, g_loss.float().contiguous(), *ctx.coefs, needs)
-        return (None, None, None, None, None, None, *grads)
+
+def _check_stats(stats, E: int, device):
+    """The statistics' tensors, a list of each kind, as the kernel reads them."""
+    kinds = [[s.expert_counts for s in stats], [s.prob_sum for s in stats], [s.lse_sq_sum for s in stats]]
+    for ts, shape, dt in zip(kinds, ((E,), (E,), (1,)), (torch.int32, torch.float32, torch.float32)):
+        assert all(t.shape == shape and t.dtype == dt and t.is_contiguous() and t.device == device for t in ts), (
+            f"statistics of {E} experts on {device}, as the fused router leaves them")
+    return kinds
 
 
 @torch.compiler.disable
@@ -221,9 +207,13 @@ def router_aux_loss(router_logits: list[torch.Tensor], num_experts: int, top_k: 
     if stats is not None:
         assert len(stats) == len(logits) and all(int(s.tokens) == lg.shape[0] for s, lg in zip(stats, logits)), (
             "one RouterStats per layer's logits, of the same rows")
-        assert all(s.expert_counts.shape == (num_experts,) and s.expert_counts.device == logits[0].device for s in stats)
-    return RouterAuxLoss(*_RouterAuxLoss.apply(ops._Layers(logits, mask), int(top_k), float(router_aux_loss_coef),
-                                               float(router_z_loss_coef), mask, stats, *logits))
+        given = _check_stats(stats, num_experts, logits[0].device)
+    else:
+        given = [], [], []
+    _check_layers(logits, mask)
+    with _stage("aux_loss"), on_device(logits[0]):
+        return RouterAuxLoss(*nodes().aux_loss(logits, mask, *given, int(top_k), float(router_aux_loss_coef),
+                                               float(router_z_loss_coef), stream_of(logits[0])))
 
 
 def _sparse_routers(model):

@@ -405,14 +405,26 @@ def test_forward_in_a_graph():
         torch.cuda.synchronize()
 
 
-def test_backward_under_capture_raises(monkeypatch):
+def test_backward_under_capture_raises():
+    """Forward and backward recorded together: the node refuses before any launch, and eager work goes on."""
     import pluggy_amd
 
     logits = draw(1, 20, 8, "fp32", 20)
-    r = pluggy_amd.router_aux_loss(logits, 8, 2)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # warm-up, eagerly
+        pluggy_amd.router_aux_loss(logits, 8, 2).loss.backward()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    want, logits[0].grad = logits[0].grad, None
+    graph = torch.cuda.CUDAGraph()
     with pytest.raises(RuntimeError, match="not supported under HIP graph capture"):
-        r.loss.backward()
+        with torch.cuda.graph(graph):
+            pluggy_amd.router_aux_loss(logits, 8, 2).loss.backward()
+    torch.cuda.synchronize()
+    logits[0].grad = None
+    pluggy_amd.router_aux_loss(logits, 8, 2).loss.backward()
+    assert torch.equal(logits[0].grad, want)
 
 
 def test_host_tensors_from_a_hook_are_refused():
@@ -438,3 +450,49 @@ def test_zeros_of_both_signs_at_the_top(E, K):
     r, grads = run(logits, K, 1.0, 0.1)
     ref = reference([torch.where(l == 0, 0.0, l)], K, 1.0, 0.1)
     check(r, grads, ref, 1.0, 0.1)
+
+
+def test_some_layers_without_gradients():
+    import pluggy_amd
+
+    logits = draw(4, 30, 16, "fp32", 27)
+    r, want = run(logits, 3, 1.0, 0.5)
+    part = [l if i in (1, 3) else l.detach() for i, l in enumerate(logits)]
+    r2 = pluggy_amd.router_aux_loss(part, 16, 3, 1.0, 0.5)
+    got = torch.autograd.grad(r2.loss, [logits[1], logits[3]])
+    assert torch.equal(r.loss, r2.loss) and torch.equal(got[0], want[1]) and torch.equal(got[1], want[3])
+    assert not r2.load_balance.requires_grad and not r2.z_loss.requires_grad
+    r3 = pluggy_amd.router_aux_loss([l.detach() for l in logits], 16, 3, 1.0, 0.5)
+    assert torch.equal(r3.loss, r.loss) and not r3.loss.requires_grad
+    with torch.no_grad():
+        assert not pluggy_amd.router_aux_loss(logits, 16, 3).loss.requires_grad
+    # the same layer twice: its gradients add up
+    twice = pluggy_amd.router_aux_loss([logits[0], logits[0]], 16, 3, 1.0, 0.5)
+    both = [logits[0].detach().clone().requires_grad_() for _ in range(2)]
+    apart = torch.autograd.grad(pluggy_amd.router_aux_loss(both, 16, 3, 1.0, 0.5).loss, both)
+    assert torch.equal(torch.autograd.grad(twice.loss, logits[0])[0], apart[0] + apart[1])
+
+
+def test_backward_twice_and_with_a_kept_graph():
+    import pluggy_amd
+
+    logits = draw(2, 20, 8, "fp32", 28)
+    loss = pluggy_amd.router_aux_loss(logits, 8, 2).loss
+    first = torch.autograd.grad(loss, logits, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, logits), first))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(loss, logits)
+    loss = pluggy_amd.router_aux_loss(logits, 8, 2).loss
+    with torch.no_grad():
+        logits[1].add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, logits)
+
+
+def test_second_derivative_is_refused():
+    import pluggy_amd
+
+    logits = draw(2, 20, 8, "fp32", 29)
+    got = torch.autograd.grad(pluggy_amd.router_aux_loss(logits, 8, 2).loss.square(), logits, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        (got[0].sum() + got[1].sum()).backward()

@@ -263,14 +263,27 @@ def test_forward_in_a_graph_and_backward_refused_there():
             torch.cuda.synchronize()
 
 
-def test_backward_under_capture_raises(monkeypatch):
+def test_backward_under_capture_raises():
+    """Forward and backward recorded together: the node refuses before any launch, and eager work goes on."""
     import pluggy_amd
 
-    x, w, b, g = inputs(8, 64, torch.float32, torch.float32, 14)
-    y = pluggy_amd.layer_norm(x.requires_grad_(), w, b)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    x, w, b, _ = inputs(8, 64, torch.float32, torch.float32, 14)
+    x.requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # warm-up, eagerly
+        pluggy_amd.layer_norm(x, w, b).sum().backward()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    want, x.grad = x.grad, None
+    graph = torch.cuda.CUDAGraph()
     with pytest.raises(RuntimeError, match="not supported under HIP graph capture"):
-        torch.autograd.grad(y, [x], g)
+        with torch.cuda.graph(graph):
+            pluggy_amd.layer_norm(x, w, b).sum().backward()
+    torch.cuda.synchronize()
+    x.grad = None
+    pluggy_amd.layer_norm(x, w, b).sum().backward()
+    assert torch.equal(x.grad, want)
 
 
 def test_second_derivative_is_refused():
@@ -329,4 +342,42 @@ def test_host_tensors_from_a_hook_are_refused():
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t):
         y = pluggy_amd.layer_norm(x.requires_grad_(), w, b)
     with pytest.raises(RuntimeError, match="ROCm GPU tensors only"):
+        torch.autograd.grad(y, [x], g)
+
+
+@pytest.mark.parametrize("which", ["x", "w", "b", "xb", "wb", "no w", "no b"])
+def test_gradients_of_any_subset(which):
+    """A gradient does not depend on which others are asked for."""
+    import pluggy_amd
+
+    x, w, b, g = inputs(40, 96, torch.float32, torch.float32, 27)
+    if which == "no w":
+        w = None
+    if which == "no b":
+        b = None
+    given = {"x": x, "w": w, "b": b}
+    full = {k: t.clone().requires_grad_() for k, t in given.items() if t is not None}
+    y = pluggy_amd.layer_norm(full["x"], full.get("w"), full.get("b"))
+    want = dict(zip(full, torch.autograd.grad(y, list(full.values()), g)))
+    names = [k for k in "xwb" if k in which] if not which.startswith("no") else ["x", "wb".replace(which[-1], "")]
+    leaves = {k: given[k].clone().requires_grad_() for k in names}
+    args = {k: leaves.get(k, t) for k, t in given.items()}
+    y = pluggy_amd.layer_norm(args["x"], args["w"], args["b"])
+    for k, got in zip(names, torch.autograd.grad(y, list(leaves.values()), g)):
+        assert torch.equal(got, want[k])
+
+
+def test_backward_twice_and_with_a_kept_graph():
+    import pluggy_amd
+
+    x, w, b, g = inputs(8, 64, torch.float32, torch.float32, 28)
+    y = pluggy_amd.layer_norm(x.requires_grad_(), w, b)
+    first = torch.autograd.grad(y, [x], g, retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(y, [x], g)[0], first)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, [x], g)
+    y = pluggy_amd.layer_norm(x, w, b)
+    with torch.no_grad():
+        x.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(y, [x], g)

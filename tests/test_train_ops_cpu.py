@@ -188,3 +188,25 @@ def test_fake_shapes_of_the_checkpointed_ops():
         assert plain[5].dtype == torch.bfloat16 and plain[6].shape == (T * K, I)
         y, stats = torch.ops.pmoe.layer_norm_fwd(torch.empty(3, 5, 8), None, None, 1e-5, torch.float16)
         assert y.shape == (3, 5, 8) and y.dtype == torch.float16 and stats.shape == (2, 15)
+
+
+def test_the_autograd_nodes_load_over_the_same_library(lib):
+    """The nodes link against the library that is loaded; one that is missing is named in the error."""
+    from pluggy_amd import _lib
+
+    assert {"layer_norm", "aux_loss"} <= set(dir(_lib.nodes()))
+    mapped = {line.split()[-1] for line in open("/proc/self/maps") if line.rstrip().endswith("libpmoe.so")}
+    assert len(mapped) == 1
+    assert lib.pmoe_stream_capturing(None) == 0
+
+
+def test_missing_autograd_nodes_are_an_error(monkeypatch):
+    import sys
+
+    from pluggy_amd import _lib
+
+    monkeypatch.setattr(_lib, "_nodes", None)
+    monkeypatch.setitem(sys.modules, "pluggy_amd._autograd", None)
+    monkeypatch.delattr("pluggy_amd._autograd", raising=False)
+    with pytest.raises(RuntimeError, match="python -m pluggy_amd.build"):
+        _lib.nodes()
