@@ -7,9 +7,9 @@
 // Both directions are bound by HBM: the forward reads x and writes y, the
 // backward reads x and g and writes gx. Rows are held in registers (the
 // variance is the mean of squared differences from the mean, not a difference
-// of two large sums), fp32 arithmetic; a row belongs to one wave up to 2048
-// columns, to two, four or eight up to 16384, and wider rows are walked by a block
-// in passes. Sums run in a fixed order, so results are deterministic.
+// of two large sums), fp32 arithmetic; a row belongs to one wave, or to two, four or
+// eight up to 16384 columns, and wider rows are walked by a block in passes. Sums
+// run in a fixed order, so results are deterministic.
 #include "kernels.h"
 #include "lanes.h"
 
@@ -169,7 +169,8 @@ __device__ __forceinline__ void row_sums(float (&v)[M], float (*s)[kLnBlock / kW
 // in registers. (Read from L1 for every row they are four times a bf16 row's
 // bytes.) Two chunks a thread leave room for four waves a SIMD, which cover each
 // other's loads; four chunks (the widest rows) for two, and there the next row is
-// on its way while a row is worked on.
+// on its way while a row is worked on. 8192 x 2048 bf16: 14.4 us, 67 MB at 4.7 TB/s;
+// 16384 x 4096: 49 us, 268 MB at 5.4; 1531 x 1001 fp32: 6.3 us; 7 x 2048: 3.5.
 template <typename TX, typename TO, int WPR, int NCH, bool VEC>
 __global__ __launch_bounds__(kLnBlock) void layernorm_fwd_kernel(const TX* __restrict__ x, const void* __restrict__ w,
                                                                  const void* __restrict__ b, int w_code, float eps,
@@ -228,10 +229,11 @@ __global__ __launch_bounds__(kLnBlock) void layernorm_fwd_kernel(const TX* __res
 
 // gx, and this block's sums of g xh and g over its rows: partial rows
 // part[2 blockIdx.x] and part[2 blockIdx.x + 1] of ld columns (part null: not
-// wanted). As in the forward the weight stays in registers and the next row is on
-// its way. The sums stay in registers too (a thread has the same columns in every
-// row), so they cost 2 * H * 8 bytes a block beside the rows' own bytes: one block
-// of eight waves a compute unit.
+// wanted). The weight stays in registers and the next row is on its way while a row
+// is worked on. The sums stay in registers too (a thread has the same columns in
+// every row), so they cost 8 H bytes a block beside the rows' own: one block of
+// eight waves a compute unit, 256 partial rows at most. 8192 x 2048 bf16: 23 us,
+// 101 MB at 4.3 TB/s; 16384 x 4096: 84 us, 403 MB at 4.8; 1531 x 1001 fp32: 9.6 us.
 template <typename TX, typename TG, int WPR, int NCH, bool VEC>
 __global__ __launch_bounds__(kLnBlock) void layernorm_bwd_kernel(const TG* __restrict__ g, const TX* __restrict__ x,
                                                                  const void* __restrict__ w, int w_code,
@@ -403,6 +405,7 @@ __global__ __launch_bounds__(kLnBlock) void layernorm_cols_kernel(const TG* __re
 
 // gw, gb = the sums of nb partial rows each, in a fixed order: 32 columns a
 // block (a lane has four), 32 groups of rows summed through LDS. No rows: zeros.
+// A latency, 4 us: 256 partial rows of 2048 columns are 4 MB, in L2 or close by.
 __global__ __launch_bounds__(256) void layernorm_reduce_kernel(const float* __restrict__ part, int nb, int64_t ld,
                                                                int H, void* __restrict__ gw, void* __restrict__ gb,
                                                                int w_code) {
@@ -433,6 +436,8 @@ bool all16(std::initializer_list<const void*> ps) {
 }
 
 // Calls f(waves a row, chunks a thread, VEC) for a row of H <= kLnRegH columns.
+// The forward: two chunks a thread, spread over more waves, against four (bf16): 7 x
+// 2048 3.5 / 4.6 us, 8192 x 2048 14.0 / 16.0, 16384 x 4096 49 / 62.
 template <class F>
 hipError_t by_width_fwd(int H, bool vec, F&& f) {
   using std::integral_constant;
