@@ -59,6 +59,17 @@ Tensor bytes(size_t n, const Tensor& like) {
   return at::empty({(int64_t)std::max<size_t>(1, n)}, like.options().dtype(at::kByte));
 }
 
+// Whether a gradient can be asked of a call on these tensors. Forward-mode derivatives are refused.
+bool differentiated(at::TensorList ts) {
+  bool any = false;
+  for (const Tensor& t : ts) {
+    if (!t.defined()) continue;
+    TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), "pmoe: forward-mode differentiation is not supported");
+    any = any || t.requires_grad();
+  }
+  return any && torch::GradMode::is_enabled();
+}
+
 // There is no second derivative: gradients that could be differentiated raise when they are.
 variable_list refuse_second(variable_list grads, const Tensor& grad) {
   if (!torch::GradMode::is_enabled() || !grad.requires_grad()) return grads;
@@ -81,18 +92,26 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     return w.defined() ? code_of(w.scalar_type()) : b.defined() ? code_of(b.scalar_type()) : PMOE_F32;
   }
 
+  // stats: (2, T) fp32, the rows' means and reciprocal deviations; undefined: not wanted.
+  static Tensor launch(const Tensor& x, const Tensor& w, const Tensor& b, double eps, at::ScalarType out_dtype,
+                       int64_t stream, const Tensor& stats) {
+    c10::DeviceGuard guard(x.device());
+    const int64_t H = x.size(-1), T = x.numel() / H;
+    Tensor out = at::empty(x.sizes(), x.options().dtype(out_dtype));
+    float* mean = stats.defined() ? stats.data_ptr<float>() : nullptr;
+    check(pmoe_layernorm_forward(data(x), code_of(x.scalar_type()), data(w), data(b), param_code(w, b), (float)eps, T,
+                                 H, data(out), code_of(out_dtype), mean, mean != nullptr ? mean + T : nullptr,
+                                 stream_of(stream)),
+          "pmoe_layernorm_forward");
+    return out;
+  }
+
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias,
                         double eps, at::ScalarType out_dtype, int64_t stream) {
     at::AutoDispatchBelowADInplaceOrView below;
-    c10::DeviceGuard guard(x.device());
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-    const int64_t H = x.size(-1), T = x.numel() / H;
-    Tensor out = at::empty(x.sizes(), x.options().dtype(out_dtype));
-    Tensor stats = at::empty({2, T}, x.options().dtype(at::kFloat));  // means, reciprocal deviations
-    float* mean = stats.data_ptr<float>();
-    check(pmoe_layernorm_forward(data(x), code_of(x.scalar_type()), data(w), data(b), param_code(w, b), (float)eps, T,
-                                 H, data(out), code_of(out_dtype), mean, mean + T, stream_of(stream)),
-          "pmoe_layernorm_forward");
+    Tensor stats = at::empty({2, x.numel() / x.size(-1)}, x.options().dtype(at::kFloat));
+    Tensor out = launch(x, w, b, eps, out_dtype, stream, stats);
     ctx->save_for_backward({x, w, b, stats});
     ctx->saved_data["stream"] = stream;
     return out;
@@ -131,7 +150,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps,
                   at::ScalarType out_dtype, int64_t stream) {
-  return LayerNorm::apply(x, weight, bias, eps, out_dtype, stream);
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  const std::array<Tensor, 3> in = {x, w, b};
+  if (differentiated(in)) return LayerNorm::apply(x, weight, bias, eps, out_dtype, stream);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return LayerNorm::launch(x, w, b, eps, out_dtype, stream, Tensor());
 }
 
 // ---------------------------------------------------- router auxiliary loss
@@ -207,6 +230,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> aux_loss(const std::vector<Tensor>& l
                                                     const std::vector<Tensor>& prob_sums,
                                                     const std::vector<Tensor>& lse_sq_sums, int64_t top_k,
                                                     double aux_coef, double z_coef, int64_t stream) {
+  const bool wanted = differentiated(logits);
   const Tensor mask = token_mask.value_or(Tensor());
   const int64_t L = (int64_t)logits.size(), E = logits[0].size(1);
   Tensor loss, balance, z, picks, coef;
@@ -240,9 +264,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> aux_loss(const std::vector<Tensor>& l
                                   coef.data_ptr<float>(), data(ws), need, stream_of(stream)),
             "pmoe_aux_loss_forward");
   }
-  bool wanted = false;
-  for (const Tensor& t : logits) wanted = wanted || t.requires_grad();
-  if (wanted && torch::GradMode::is_enabled()) {
+  if (wanted) {
     std::shared_ptr<AuxLossBackward> node(new AuxLossBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(at::TensorList(logits)));
     node->logits.reserve(L);
@@ -260,6 +282,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> aux_loss(const std::vector<Tensor>& l
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
-  m.def("aux_loss", &aux_loss, py::call_guard<py::gil_scoped_release>());
+  // errors come out as torch's own classes (out of memory among them), a hook's as they were raised
+  m.def("layer_norm", torch::wrap_pybind_function_no_gil(layer_norm));
+  m.def("aux_loss", torch::wrap_pybind_function_no_gil(aux_loss));
 }

@@ -2,10 +2,10 @@
 
 ``layer_norm`` is ``torch.nn.functional.layer_norm`` over the last dimension,
 forward and backward, in fp32 arithmetic; ``moe_sublayer`` calls it for a block
-whose norm is a ``torch.nn.LayerNorm``. Eager calls go through one autograd node
-in C++ (``csrc/autograd.cpp``; where no gradient is wanted, straight to the
-kernel); under ``torch.compile`` they are the custom ops ``pmoe::layer_norm_fwd``
-and ``pmoe::layer_norm_bwd``, which trace without graph breaks.
+whose norm is a ``torch.nn.LayerNorm``. Eager calls are one autograd node in C++
+(``csrc/autograd.cpp``); under ``torch.compile`` they are the custom ops
+``pmoe::layer_norm_fwd`` and ``pmoe::layer_norm_bwd``, which trace without graph
+breaks.
 """
 
 from __future__ import annotations
@@ -75,8 +75,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     types are both taken in fp32. The result has ``x``'s type, or ``out_dtype``
     (16 bits from fp32 ``x``: what the 16-bit products of the block read, without
     a cast between). Unlike torch's, it does not follow autocast. Gradients reach
-    ``x`` and the parameters; a second derivative is refused, and so is a
-    backward under HIP graph capture.
+    ``x`` and the parameters; a second derivative and forward-mode differentiation are
+    refused, and so is a backward under HIP graph capture.
     """
     assert x.dim() >= 1 and x.shape[-1] >= 1, "layer_norm expects (..., H)"
     H = x.shape[-1]
@@ -91,8 +91,5 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     x, weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (x, weight, bias))
     if torch.compiler.is_compiling():
         return torch.ops.pmoe.layer_norm_fwd(x, weight, bias, float(eps), out_dtype)[0]
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in (x, weight, bias)]):
-        with _stage("layernorm"), on_device(x):
-            return nodes().layer_norm(x, weight, bias, float(eps), out_dtype, stream_of(x))
-    with _stage("layernorm"):
-        return ops.layernorm_forward(x, weight, bias, float(eps), out_dtype, stats=False)[0]
+    with _stage("layernorm"), on_device(x):
+        return nodes().layer_norm(x, weight, bias, float(eps), out_dtype, stream_of(x))

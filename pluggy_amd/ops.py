@@ -348,10 +348,10 @@ def dispatch_rmsnorm_backward(grad_x_perm, inv_pos, grad_normed_add, x, weight, 
 # ------------------------------------------------------------------ layer norm
 
 
-def layernorm_forward(x, weight, bias, eps: float, out_dtype, stats: bool = True):
+def layernorm_forward(x, weight, bias, eps: float, out_dtype):
     """torch.nn.LayerNorm over the last dimension of x (..., H) in fp32 arithmetic -> out (..., H) out_dtype
-    and stats (2, T) fp32, the T rows' means and reciprocal deviations (None without ``stats``). weight and
-    bias (H,), one dtype, or None."""
+    and stats (2, T) fp32, the T rows' means and reciprocal deviations. weight and bias (H,), one dtype, or
+    None."""
     require_gpu(x, weight, bias)
     H = x.shape[-1]
     T = x.numel() // H
@@ -360,12 +360,12 @@ def layernorm_forward(x, weight, bias, eps: float, out_dtype, stats: bool = True
     assert weight is None or bias is None or weight.dtype == bias.dtype
     wdt = next((p.dtype for p in (weight, bias) if p is not None), torch.float32)
     out = torch.empty_like(x, dtype=out_dtype)
-    kept = torch.empty(2, T, dtype=torch.float32, device=x.device) if stats else None
-    mean = ptr(kept) if stats else None
+    stats = torch.empty(2, T, dtype=torch.float32, device=x.device)
+    mean = stats.data_ptr()
     with on_device(x):
         call("pmoe_layernorm_forward", ptr(x), dtype_code(x.dtype), ptr(weight), ptr(bias), dtype_code(wdt),
-             float(eps), T, H, ptr(out), dtype_code(out_dtype), mean, mean + 4 * T if stats else None, stream_of(x))
-    return out, kept
+             float(eps), T, H, ptr(out), dtype_code(out_dtype), mean, mean + 4 * T, stream_of(x))
+    return out, stats
 
 
 def layernorm_backward(grad, x, weight, stats, weight_dtype=torch.float32, need_x: bool = True,

@@ -185,8 +185,8 @@ def router_aux_loss(router_logits: list[torch.Tensor], num_experts: int, top_k: 
     then come from them without a pass over the logits. They cover every row, so
     they do not go with a mask.
 
-    Runs eagerly inside ``torch.compile`` (a graph break). A second derivative and a backward
-    under HIP graph capture are refused.
+    Runs eagerly inside ``torch.compile`` (a graph break). A second derivative,
+    forward-mode differentiation and a backward under HIP graph capture are refused.
     """
     logits = [router_logits] if isinstance(router_logits, torch.Tensor) else list(router_logits)
     if not logits:

@@ -496,3 +496,29 @@ def test_second_derivative_is_refused():
     got = torch.autograd.grad(pluggy_amd.router_aux_loss(logits, 8, 2).loss.square(), logits, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivative"):
         (got[0].sum() + got[1].sum()).backward()
+
+
+def test_under_activation_checkpointing():
+    from torch.utils.checkpoint import checkpoint
+
+    import pluggy_amd
+
+    logits = draw(3, 40, 16, "fp32", 30)
+
+    def f(*ls):
+        return pluggy_amd.router_aux_loss([l * 2 for l in ls], 16, 2, 1.0, 0.1).loss
+
+    want = torch.autograd.grad(f(*logits), logits)
+    got = torch.autograd.grad(checkpoint(f, *logits, use_reentrant=False), logits)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+
+    import pluggy_amd
+
+    l = torch.randn(20, 8, device=DEV)
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            pluggy_amd.router_aux_loss([fw.make_dual(l, torch.ones_like(l))], 8, 2)

@@ -381,3 +381,49 @@ def test_backward_twice_and_with_a_kept_graph():
         x.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(y, [x], g)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_under_activation_checkpointing(reentrant):
+    """Computed again in the backward, where the second forward stops as soon as what is needed is there."""
+    from torch.utils.checkpoint import checkpoint
+
+    import pluggy_amd
+
+    x, w, b, g = inputs(40, 96, torch.float32, torch.float32, 29)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+
+    def f(x, w, b):
+        return pluggy_amd.layer_norm(x * 2, w, b).sin()
+
+    want = torch.autograd.grad(f(*leaves), leaves, g)
+    if reentrant:
+        checkpoint(f, *leaves, use_reentrant=True).backward(g)
+        got = [t.grad for t in leaves]
+    else:
+        got = torch.autograd.grad(checkpoint(f, *leaves, use_reentrant=False), leaves, g)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+
+    import pluggy_amd
+
+    x = torch.randn(4, 64, device=DEV)
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            pluggy_amd.layer_norm(fw.make_dual(x, torch.ones_like(x)))
+
+
+def test_without_gradients_the_same_values():
+    import pluggy_amd
+
+    x, w, b, _ = inputs(33, 257, torch.float32, torch.float32, 30)
+    want = pluggy_amd.layer_norm(x.clone().requires_grad_(), w, b).detach()
+    assert torch.equal(pluggy_amd.layer_norm(x, w, b), want)
+    with torch.no_grad():
+        y = pluggy_amd.layer_norm(x.requires_grad_(), w, b)
+    assert torch.equal(y, want) and not y.requires_grad
+    with torch.inference_mode():
+        assert torch.equal(pluggy_amd.layer_norm(x.detach(), w, b), want)
