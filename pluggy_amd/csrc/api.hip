@@ -1156,7 +1156,7 @@ PMOE_API int pmoe_layernorm_forward(const void* x, int x_dtype, const void* weig
 
 PMOE_API size_t pmoe_layernorm_backward_workspace_size(int64_t T, int64_t H) {
   if (T <= 0 || H <= 0 || H > (int64_t)1 << 30 || T > layernorm_max_rows((int)H)) return 0;
-  return align_up((size_t)2 * layernorm_bwd_blocks(T, (int)H) * layernorm_part_ld((int)H) * sizeof(float));
+  return align_up((size_t)2 * layernorm_bwd_blocks(T, (int)H, true) * layernorm_part_ld((int)H) * sizeof(float));
 }
 
 PMOE_API int pmoe_layernorm_backward(const void* grad, int grad_dtype, const void* x, int x_dtype, const void* weight,

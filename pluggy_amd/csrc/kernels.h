@@ -153,12 +153,12 @@ hipError_t sum_row_groups(const float* partial, int rows, int n, float* tmp, hip
 template <typename TX, typename TO>
 hipError_t layernorm_fwd(const TX* x, const void* w, const void* b, int w_code, float eps, int64_t T_, int H, TO* out,
                          float* mean, float* rstd, hipStream_t s);
-// gx, gw and gb may each be null; part: 2 * layernorm_bwd_blocks(T, H) rows of
+// gx, gw and gb may each be null; part: 2 * layernorm_bwd_blocks(T, H, half) rows of
 // layernorm_part_ld(H) floats, 16-byte aligned (null when neither gw nor gb is wanted).
 template <typename TX, typename TG>
 hipError_t layernorm_bwd(const TG* g, const TX* x, const void* w, int w_code, const float* mean, const float* rstd,
                          int64_t T_, int H, TX* gx, float* part, void* gw, void* gb, hipStream_t s);
-int layernorm_bwd_blocks(int64_t T_, int H);
+int layernorm_bwd_blocks(int64_t T_, int H, bool half);  // half: 16-bit x (as many blocks as fp32, or more)
 int64_t layernorm_part_ld(int H);
 int64_t layernorm_max_rows(int H);
 

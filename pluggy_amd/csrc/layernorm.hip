@@ -18,7 +18,8 @@ namespace {
 
 constexpr int kLnBlock = 512;       // threads of a block
 constexpr int kLnRegH = 16384;      // widest row held in registers
-constexpr int kLnMaxBlocks = 256;   // blocks (partial rows) of the backward: one a compute unit
+constexpr int kLnMaxBlocks = 256;   // blocks (partial rows) of the backward: one a compute unit, ...
+constexpr int kLnTwoH = 2048;       // ... two for 16-bit rows up to this width
 constexpr int kLnFwdBlocks = 768;   // most blocks of the forward: three a compute unit
 constexpr int kLnColBlocks = 1024;  // most row chunks of the wide rows' column sums, ...
 constexpr int kLnColRows = 256;     // each of at least so many rows
@@ -231,9 +232,9 @@ __global__ __launch_bounds__(kLnBlock) void layernorm_fwd_kernel(const TX* __res
 // part[2 blockIdx.x] and part[2 blockIdx.x + 1] of ld columns (part null: not
 // wanted). The weight stays in registers and the next row is on its way while a row
 // is worked on. The sums stay in registers too (a thread has the same columns in
-// every row), so they cost 8 H bytes a block beside the rows' own: one block of
-// eight waves a compute unit, 256 partial rows at most. 8192 x 2048 bf16: 23 us,
-// 101 MB at 4.3 TB/s; 16384 x 4096: 84 us, 403 MB at 4.8; 1531 x 1001 fp32: 9.6 us.
+// every row), so they cost 8 H bytes a block beside the rows' own: one or two
+// blocks of eight waves a compute unit, no more. 8192 x 2048 bf16: 21.5 us, 101 MB
+// at 4.7 TB/s; 16384 x 4096: 84 us, 403 MB at 4.8; 1531 x 1001 fp32: 9.6 us.
 template <typename TX, typename TG, int WPR, int NCH, bool VEC>
 __global__ __launch_bounds__(kLnBlock) void layernorm_bwd_kernel(const TG* __restrict__ g, const TX* __restrict__ x,
                                                                  const void* __restrict__ w, int w_code,
@@ -449,22 +450,26 @@ hipError_t by_width_fwd(int H, bool vec, F&& f) {
   if (H <= 8192) return go(integral_constant<int, 8>(), integral_constant<int, 2>());
   return go(integral_constant<int, 8>(), integral_constant<int, 4>());
 }
-// The backward holds six values a column: `narrow` (fp32 rows, and rows whose last
-// chunk may be cut) in two chunks a thread, where four would spill. 8192 x 2048,
-// narrow / four chunks: fp32 38 / 42 us, fp32 with bf16 gradients 33 / 37, bf16
-// 26.7 / 26.7 (16384 x 4096 82 / 80, 4096 x 8192 46 / 45).
+// The backward holds six values a column, in two chunks a thread up to 2048 columns
+// and beyond them for `narrow` rows (fp32, or a last chunk that may be cut), where
+// four would spill: 8192 x 2048 fp32, two / four chunks 38 / 42 us, fp32 with bf16
+// gradients 33 / 37; 4096 x 8192 bf16 46 / 45.
+// 16-bit rows in two chunks leave room for two blocks a compute unit. Two / one (of
+// four chunks from 1025 columns on), with the sums' launch, bf16: 32768 x 512 24.0 /
+// 26.9 us, 32768 x 1024 40.4 / 42.1, 2048 x 2048 14.0 / 16.2, 8192 x 2048 25.4 / 27.5,
+// 8192 x 2001 26.0 / 31.1; but 16384 x 4096 82 / 80, 4096 x 8192 53 / 44, and fp32,
+// whose registers do not fit, 8192 x 2048 42 / 39.
 template <class F>
 hipError_t by_width_bwd(int H, bool vec, bool narrow, F&& f) {
   using std::integral_constant;
   auto go = [&](auto wpr, auto nch) { return vec ? f(wpr, nch, std::true_type()) : f(wpr, nch, std::false_type()); };
   if (H <= 512) return go(integral_constant<int, 1>(), integral_constant<int, 1>());
   if (H <= 1024) return go(integral_constant<int, 1>(), integral_constant<int, 2>());
+  if (H <= 2048) return go(integral_constant<int, 2>(), integral_constant<int, 2>());
   if (narrow) {
-    if (H <= 2048) return go(integral_constant<int, 2>(), integral_constant<int, 2>());
     if (H <= 4096) return go(integral_constant<int, 4>(), integral_constant<int, 2>());
     if (H <= 8192) return go(integral_constant<int, 8>(), integral_constant<int, 2>());
   } else {
-    if (H <= 2048) return f(integral_constant<int, 1>(), integral_constant<int, 4>(), std::true_type());
     if (H <= 4096) return f(integral_constant<int, 2>(), integral_constant<int, 4>(), std::true_type());
     if (H <= 8192) return f(integral_constant<int, 4>(), integral_constant<int, 4>(), std::true_type());
   }
@@ -477,11 +482,11 @@ int64_t wide_rows(int64_t T_) { return std::max<int64_t>(kLnColRows, (T_ + kLnCo
 
 }  // namespace
 
-int layernorm_bwd_blocks(int64_t T_, int H) {
+int layernorm_bwd_blocks(int64_t T_, int H, bool half) {
   if (T_ <= 0) return 0;
   if (H > kLnRegH) return (int)((T_ + wide_rows(T_) - 1) / wide_rows(T_));
   const int rpb = rows_a_block(H);
-  return (int)std::min<int64_t>((T_ + rpb - 1) / rpb, kLnMaxBlocks);
+  return (int)std::min<int64_t>((T_ + rpb - 1) / rpb, half && H <= kLnTwoH ? 2 * kLnMaxBlocks : kLnMaxBlocks);
 }
 
 int64_t layernorm_part_ld(int H) { return ln_pad(H); }
@@ -513,7 +518,7 @@ template <typename TX, typename TG>
 hipError_t layernorm_bwd(const TG* g, const TX* x, const void* w, int w_code, const float* mean, const float* rstd,
                          int64_t T_, int H, TX* gx, float* part, void* gw, void* gb, hipStream_t s) {
   const bool vec = H % 8 == 0 && all16({g, x, w, gx, part});
-  const int nb = layernorm_bwd_blocks(T_, H);
+  const int nb = layernorm_bwd_blocks(T_, H, sizeof(TX) == 2);
   const int64_t ld = layernorm_part_ld(H);
   hipError_t st = hipSuccess;
   if (T_ > 0 && H > kLnRegH) {
