@@ -415,3 +415,51 @@ def test_a_training_step_of_all_together():
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][2], got[1][2])
     for a, b in zip(got[0][1], got[1][1]):
         assert (a - b).norm() <= 0.05 * a.norm() and a.norm() > 0
+
+
+def test_in_a_graph_and_on_another_stream():
+    """Saving, restoring and the GEMMs around the checkpoint, replayed on changed inputs with eager work between."""
+    import pluggy_amd
+    from pluggy_amd import ops
+
+    mlp = pluggy_amd.Qwen3MoeSparseMLP(64, 48, 8, 2).to(DEV).to(torch.bfloat16)
+    mlp.experts.checkpoint_8bit = True
+    g = gen(91)
+    with torch.no_grad():
+        for p in mlp.parameters():
+            p.copy_((torch.randn(p.shape, generator=g) * 0.1).to(DEV))
+    x = torch.randn(1, 300, 64, generator=g).to(torch.bfloat16).to(DEV)
+
+    def step():
+        codes, exps = ops.act8_save(x)
+        return ops.act8_restore(codes, exps, torch.bfloat16), codes, exps, mlp(x).detach()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(on_side, step()))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(3):
+        x.mul_(1.5)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+        torch.cuda.synchronize()
+
+
+def test_past_32_bit_offsets():
+    """2.2e9 values: the last rows are those of the rows by themselves."""
+    from pluggy_amd import ops
+
+    R, C = 1100000, 2000
+    x = torch.randn(R, C, device=DEV, dtype=torch.bfloat16)
+    codes, exps = ops.act8_save(x)
+    back = ops.act8_restore(codes, exps, torch.bfloat16)
+    for rows in (slice(0, 40), slice(R - 40, R)):
+        c, e = ops.act8_save(x[rows])
+        assert torch.equal(codes[rows], c) and torch.equal(exps[rows], e)
+        assert torch.equal(back[rows], ops.act8_restore(c, e, torch.bfloat16))

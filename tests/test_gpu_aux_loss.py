@@ -522,3 +522,23 @@ def test_forward_mode_is_refused():
     with fw.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             pluggy_amd.router_aux_loss([fw.make_dual(l, torch.ones_like(l))], 8, 2)
+
+
+def test_past_32_bit_offsets():
+    """2.2e9 logits: all rows counted, the last rows' gradients by the formula with the counts at hand."""
+    import pluggy_amd
+
+    N, E, K = 18000000, 128, 8
+    l = torch.randn(N, E, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    r = pluggy_amd.router_aux_loss([l], E, K, 1.0, 1.0)
+    (g,) = torch.autograd.grad(r.loss * N, [l])
+    assert r.expert_counts.sum().item() == N * K
+    f = r.expert_counts[0].double() / N - K / E
+    for rows in (slice(0, 64), slice(N - 64, N)):
+        p = torch.softmax(l[rows].detach().double(), -1)
+        lse = torch.logsumexp(l[rows].detach().double(), -1)[:, None]
+        m = (p * f).sum(-1, keepdim=True)
+        want = p * (E * (f - m) + 2 * lse)
+        bound = 96 * U * p * (E * (f.abs() + m.abs()) + 2 * (lse.abs() + 1))
+        bound = bound + (want.abs() + bound) * torch.finfo(torch.bfloat16).eps / 2
+        assert ((g[rows].double() - want).abs() <= bound + torch.finfo(torch.bfloat16).tiny).all()

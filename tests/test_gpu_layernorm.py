@@ -427,3 +427,21 @@ def test_without_gradients_the_same_values():
     assert torch.equal(y, want) and not y.requires_grad
     with torch.inference_mode():
         assert torch.equal(pluggy_amd.layer_norm(x.detach(), w, b), want)
+
+
+@pytest.mark.parametrize("H", [2001, 17000])
+def test_past_32_bit_offsets(H):
+    """2.2e9 values, held in registers and walked in passes: the last rows are those of the rows by themselves."""
+    import pluggy_amd
+
+    T = 2200000000 // H
+    x = torch.randn(T, H, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    w, b = torch.rand(H, device=DEV) + 0.5, torch.randn(H, device=DEV)
+    g = torch.randn(T, H, device=DEV, dtype=torch.bfloat16)
+    y = pluggy_amd.layer_norm(x, w, b)
+    gx = torch.autograd.grad(y, [x], g)[0]
+    for rows in (slice(0, 40), slice(T - 40, T)):
+        part = x[rows].detach().requires_grad_()
+        yp = pluggy_amd.layer_norm(part, w, b)
+        assert torch.equal(y[rows], yp)
+        assert torch.equal(gx[rows], torch.autograd.grad(yp, [part], g[rows])[0])
