@@ -640,8 +640,8 @@ hipError_t aux_finish(const float* psum, const int32_t* part_counts, const float
                       uint32_t* arrived, const AuxOut& out, hipStream_t s) {
   // One block while it reads the partial sums in a few microseconds; several need
   // device-wide fences between them. One / several, us: 6 layers of 60 experts 6.7 /
-  // 12.6; 48 of 128 (30720 partial sums) 11.6 / 12.5; 128 of 128 (65536) 19.6 / 15.1;
-  // 48 of 256 (61440) 18.1 / 13.0.
+  // 12.6; 48 of 128 (just under 2^15 sums) 11.6 / 12.5; 128 of 128 (2^16) 19.6 / 15.1;
+  // 48 of 256 (just under 2^16) 18.1 / 13.0.
   int cols = kCols;
   if (E <= 256 && (int64_t)L * bpl * E <= kAuxOneBlock)
     while (cols < E) cols *= 2;
