@@ -338,8 +338,9 @@ PMOE_API int pmoe_expert_ffn_backward(const void* grad_out, const void* hidden, 
  * the number of valid rows:
  *   LB = E sum_e (c_e / n) (sum_t p_te / n),   Z = sum_t lse_t^2 / n,
  *   loss = aux_coef LB + z_coef Z, load_balance = LB, z_loss = Z
- * (one fp32 each in device memory). No valid row: all three are 0. logits: a HOST array of L device pointers, each
- * (rows[i], E) of `dtype` (fp32, bf16 or fp16), row_counts a HOST array of L.
+ * (one fp32 each in device memory). No valid row: all three are 0. logits: a HOST
+ * array of L device pointers (1 <= L <= 4096), each (row_counts[i], E) of `dtype`
+ * (fp32, bf16 or fp16), row_counts a HOST array of L.
  * mask: (mask_rows,) bytes or NULL; a row whose byte is 0 counts for nothing,
  * whatever it holds, in every layer (each then has mask_rows rows).
  * expert_counts: (L, E) int32; coef: (E + 1,) fp32 that the backward takes. The
@@ -347,8 +348,9 @@ PMOE_API int pmoe_expert_ffn_backward(const void* grad_out, const void* hidden, 
 PMOE_API size_t pmoe_aux_loss_forward_workspace_size(const int64_t* row_counts, int64_t L, int64_t E);
 PMOE_API int pmoe_aux_loss_forward(const void* const* logits, const int64_t* row_counts, int64_t L, int dtype,
                                    const uint8_t* mask, int64_t mask_rows, int64_t E, int64_t K, float aux_coef,
-                                   float z_coef, float* loss, float* load_balance, float* z_loss, int32_t* expert_counts, float* coef, void* workspace,
-                                   size_t workspace_bytes, void* stream);
+                                   float z_coef, float* loss, float* load_balance, float* z_loss,
+                                   int32_t* expert_counts, float* coef, void* workspace, size_t workspace_bytes,
+                                   void* stream);
 
 /* The same values from the statistics that pmoe_router_forward emits (no pass
  * over the logits): HOST arrays of L device pointers to each layer's
@@ -357,8 +359,9 @@ PMOE_API int pmoe_aux_loss_forward(const void* const* logits, const int64_t* row
 PMOE_API size_t pmoe_aux_loss_from_stats_workspace_size(int64_t L, int64_t E);
 PMOE_API int pmoe_aux_loss_from_stats(const int32_t* const* layer_counts, const float* const* prob_sums,
                                       const float* const* lse_sq_sums, int64_t L, int64_t n, int64_t E, int64_t K,
-                                      float aux_coef, float z_coef, float* loss, float* load_balance, float* z_loss, int32_t* expert_counts, float* coef,
-                                      void* workspace, size_t workspace_bytes, void* stream);
+                                      float aux_coef, float z_coef, float* loss, float* load_balance, float* z_loss,
+                                      int32_t* expert_counts, float* coef, void* workspace, size_t workspace_bytes,
+                                      void* stream);
 
 /* Gradient of loss times grad_loss (1,) fp32 in device memory: into
  * grads[i] (HOST array of L device pointers; NULL: not wanted), shaped and typed

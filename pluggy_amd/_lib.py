@@ -62,7 +62,8 @@ SIGNATURES = {
     "pmoe_aux_loss_forward": (_INT, [_P, _P, _I64, _INT, _P, _I64, _I64, _I64, _F32, _F32, _P, _P, _P, _P, _P, _P, _SZ,
                                      _P]),
     "pmoe_aux_loss_from_stats_workspace_size": (_SZ, [_I64, _I64]),
-    "pmoe_aux_loss_from_stats": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _F32, _F32, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "pmoe_aux_loss_from_stats": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _F32, _F32, _P, _P, _P, _P, _P, _P, _SZ,
+                                        _P]),
     "pmoe_aux_loss_backward": (_INT, [_P, _P, _P, _I64, _INT, _P, _I64, _I64, _P, _P, _F32, _F32, _P]),
     "pmoe_layernorm_forward": (_INT, [_P, _INT, _P, _P, _INT, _F32, _I64, _I64, _P, _INT, _P, _P, _P]),
     "pmoe_layernorm_backward_workspace_size": (_SZ, [_I64, _I64]),

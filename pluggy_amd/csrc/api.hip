@@ -1011,8 +1011,9 @@ PMOE_API size_t pmoe_aux_loss_forward_workspace_size(const int64_t* row_counts, 
 
 PMOE_API int pmoe_aux_loss_forward(const void* const* logits, const int64_t* row_counts, int64_t L, int dtype,
                                    const uint8_t* mask, int64_t mask_rows, int64_t E, int64_t K, float aux_coef,
-                                   float z_coef, float* loss, float* load_balance, float* z_loss, int32_t* expert_counts, float* coef, void* workspace,
-                                   size_t workspace_bytes, void* stream) {
+                                   float z_coef, float* loss, float* load_balance, float* z_loss,
+                                   int32_t* expert_counts, float* coef, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
   AuxPlan plan;
   if (int rc = check_aux(logits, row_counts, L, E, K, "aux_loss_forward", &plan)) return rc;
   if (int rc = check_mask(mask, mask_rows, row_counts, L, "aux_loss_forward")) return rc;
@@ -1052,8 +1053,9 @@ PMOE_API size_t pmoe_aux_loss_from_stats_workspace_size(int64_t L, int64_t E) {
 
 PMOE_API int pmoe_aux_loss_from_stats(const int32_t* const* layer_counts, const float* const* prob_sums,
                                       const float* const* lse_sq_sums, int64_t L, int64_t n, int64_t E, int64_t K,
-                                      float aux_coef, float z_coef, float* loss, float* load_balance, float* z_loss, int32_t* expert_counts, float* coef,
-                                      void* workspace, size_t workspace_bytes, void* stream) {
+                                      float aux_coef, float z_coef, float* loss, float* load_balance, float* z_loss,
+                                      int32_t* expert_counts, float* coef, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
   PMOE_REQUIRE(L >= 1 && L <= 4096, "aux_loss_from_stats: %lld layers (1 to 4096 are supported)", (long long)L);
   if (int rc = check_moe_dims(0, K, E, 8, 0)) return rc;
   PMOE_REQUIRE(n >= 0 && n <= kMaxIndex, "aux_loss_from_stats: %lld rows", (long long)n);
@@ -1112,7 +1114,6 @@ PMOE_API int pmoe_aux_loss_backward(const void* const* logits, void* const* grad
 
 extern "C++" {
 namespace {
-
 
 int check_layernorm(int64_t T, int64_t H, int x_dtype, int w_dtype, int y_dtype, const char* what) {
   PMOE_REQUIRE(T >= 0 && T <= kMaxIndex && H > 0 && H <= (int64_t)1 << 30, "%s: bad sizes T=%lld H=%lld", what,

@@ -609,7 +609,10 @@ hipError_t by_experts(int E, uintptr_t low, F&& f) {
 
 uintptr_t low_bits(const AuxLayers& a, const AuxGrads* g, int L) {
   uintptr_t low = 0;
-  for (int i = 0; i < L; ++i) low |= reinterpret_cast<uintptr_t>(a.logits[i]) | (g != nullptr ? reinterpret_cast<uintptr_t>(g->grad[i]) : 0);
+  for (int i = 0; i < L; ++i) {
+    low |= reinterpret_cast<uintptr_t>(a.logits[i]);
+    if (g != nullptr) low |= reinterpret_cast<uintptr_t>(g->grad[i]);
+  }
   return low;
 }
 
@@ -630,7 +633,8 @@ hipError_t aux_stats(const AuxLayers& layers, int L, const uint8_t* mask, int E,
                      int32_t* counts, float* lse2, int32_t* rows, uint32_t* arrived, hipStream_t s) {
   return by_experts<T>(E, low_bits(layers, nullptr, L), [&](auto lpr, auto v, auto w) {
     hipLaunchKernelGGL((aux_stats_kernel<T, decltype(lpr)::value, decltype(v)::value, decltype(w)::value>),
-                       dim3(bpl, L), dim3(stats_block(decltype(lpr)::value * decltype(v)::value)), 0, s, layers, mask, E, K, psum, counts, lse2, rows, arrived);
+                       dim3(bpl, L), dim3(stats_block(decltype(lpr)::value * decltype(v)::value)), 0, s, layers, mask,
+                       E, K, psum, counts, lse2, rows, arrived);
     return hipGetLastError();
   });
 }
@@ -673,7 +677,7 @@ hipError_t aux_grad(const AuxLayers& layers, const AuxGrads& grads, int L, int64
 
 #define PMOE_INST_AUX(T)                                                                                             \
   template hipError_t aux_stats<T>(const AuxLayers&, int, const uint8_t*, int, int, int, float*, int32_t*, float*,   \
-                                   int32_t*, uint32_t*, hipStream_t);                                                           \
+                                   int32_t*, uint32_t*, hipStream_t);                                                \
   template hipError_t aux_grad<T>(const AuxLayers&, const AuxGrads&, int, int64_t, const uint8_t*, int,              \
                                   const float*, const float*, float, float, hipStream_t);
 PMOE_INST_AUX(float)

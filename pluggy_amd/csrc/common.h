@@ -5,6 +5,8 @@
 #include <stdint.h>
 #include <stddef.h>
 
+#include <type_traits>
+
 namespace pmoe {
 
 typedef uint16_t bf16_t;  // bf16 storage: the upper 16 bits of an fp32
@@ -216,6 +218,37 @@ template <> struct Fmt16<f16_t> {
   __device__ static __forceinline__ float lo(uint32_t w) { return f16lo(w); }
   __device__ static __forceinline__ float hi(uint32_t w) { return f16hi(w); }
 };
+
+// 16 bytes at any element's alignment (the memory path takes unaligned vector accesses).
+typedef u32x4 u32x4_by2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_by4 __attribute__((aligned(4)));
+template <typename T> struct Loose { typedef std::conditional_t<sizeof(T) == 2, u32x4_by2, u32x4_by4> type; };
+
+// Vec8's load and store at any element's alignment.
+template <typename T>
+__device__ __forceinline__ void load8_loose(const T* p, float* v) {
+  const typename Loose<T>::type* q = reinterpret_cast<const typename Loose<T>::type*>(p);
+  if constexpr (sizeof(T) == 4) {
+    const u32x4 lo = q[0], hi = q[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(lo[i]); v[4 + i] = __uint_as_float(hi[i]); }
+  } else {
+    const u32x4 w = q[0];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = Fmt16<T>::lo(w[i]); v[2 * i + 1] = Fmt16<T>::hi(w[i]); }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8_loose(T* p, const float* v) {
+  typename Loose<T>::type* q = reinterpret_cast<typename Loose<T>::type*>(p);
+  if constexpr (sizeof(T) == 4) {
+    q[0] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    q[1] = u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+  } else {
+    q[0] = u32x4{Fmt16<T>::pack2(v[0], v[1]), Fmt16<T>::pack2(v[2], v[3]), Fmt16<T>::pack2(v[4], v[5]),
+                 Fmt16<T>::pack2(v[6], v[7])};
+  }
+}
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 

@@ -34,11 +34,6 @@ __device__ __forceinline__ float param(const void* p, int code, int c, float non
   return (float)static_cast<const f16_t*>(p)[c];
 }
 
-// 16 bytes at any element's alignment (the memory path takes unaligned vector accesses).
-typedef u32x4 u32x4_by2 __attribute__((aligned(2)));
-typedef u32x4 u32x4_by4 __attribute__((aligned(4)));
-template <typename T> struct Loose { typedef std::conditional_t<sizeof(T) == 2, u32x4_by2, u32x4_by4> type; };
-
 // Eight of them from column c on; LOOSE: at any element's alignment.
 template <bool LOOSE>
 __device__ __forceinline__ void param8(const void* p, int code, int c, float none, float* v) {
@@ -77,17 +72,7 @@ struct Cols {
     if constexpr (VEC) {
       Vec8<T>::store(row + c, v);
     } else if (c + 8 <= H) {
-      typedef typename Loose<T>::type P;
-      if constexpr (sizeof(T) == 4) {
-        const u32x4 lo = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-        const u32x4 hi = {__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
-        *reinterpret_cast<P*>(row + c) = lo;
-        *reinterpret_cast<P*>(row + c + 4) = hi;
-      } else {
-        const u32x4 w = {Fmt16<T>::pack2(v[0], v[1]), Fmt16<T>::pack2(v[2], v[3]), Fmt16<T>::pack2(v[4], v[5]),
-                         Fmt16<T>::pack2(v[6], v[7])};
-        *reinterpret_cast<P*>(row + c) = w;
-      }
+      store8_loose<T>(row + c, v);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
