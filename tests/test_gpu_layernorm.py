@@ -445,3 +445,43 @@ def test_past_32_bit_offsets(H):
         yp = pluggy_amd.layer_norm(part, w, b)
         assert torch.equal(y[rows], yp)
         assert torch.equal(gx[rows], torch.autograd.grad(yp, [part], g[rows])[0])
+
+
+def test_from_several_threads_on_their_own_streams():
+    """Calls at once: each thread's results are those of the same work alone."""
+    import threading
+
+    import pluggy_amd
+
+    def work(k):
+        x, w, b, g = inputs(200 + k, 333, torch.float32, torch.float32, 40 + k)
+        leaves = [t.requires_grad_() for t in (x, w, b)]
+        logits = [torch.randn(100 + k, 24, generator=gen(50 + k)).to(DEV).requires_grad_() for _ in range(3)]
+        out = []
+        for _ in range(10):
+            y = pluggy_amd.layer_norm(*leaves)
+            r = pluggy_amd.router_aux_loss(logits, 24, 3, 1.0, 0.1)
+            out.append([y, r.loss, *torch.autograd.grad(y, leaves, g), *torch.autograd.grad(r.loss, logits)])
+        return out
+
+    alone = [work(k) for k in range(4)]
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def run(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                got[k] = work(k)
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for k in range(4):
+        assert all(torch.equal(a, b) for u, v in zip(got[k], alone[k]) for a, b in zip(u, v))
