@@ -7,8 +7,8 @@
 // bf16, 305 MB each way: saving 57 us, restoring 64, 5.4 and 4.8 TB/s, what a large
 // copy reaches (5.1). Stores stay cached: non-temporal ones restore faster in a row
 // (67 -> 47), but whatever reads the result next pays for it (96 MB, restoring and
-// then reading: 38 + 31 us cached, 35 + 52 not). The MoE's own checkpoint needs neither launch: the GEMM
-// epilogues write and read the codes (gemm_persist.h).
+// then reading: 38 + 31 us cached, 35 + 52 not). The MoE's own checkpoint needs
+// neither launch: the GEMM epilogues write and read the codes (gemm_persist.h).
 #include "act8.h"
 #include "kernels.h"
 
