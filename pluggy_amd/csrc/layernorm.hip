@@ -88,7 +88,11 @@ struct Cols {
       for (int e = 0; e < 8; ++e) v[e] = c + e < H ? param(p, code, c + e, none) : 0.0f;
     }
   }
-  // A row's chunks as read, to be unpacked when they are used.
+  // A row's chunks as read, to be unpacked when they are used. The one that the row's
+  // end cuts is read as the row's last 8 elements and moved down then, so that no
+  // load is waited for before its use. Against reading it element by element, bf16,
+  // forward and backward: 32768 x 511 20 + 39 -> 18 + 28 us, 8192 x 2001 13.5 + 25 ->
+  // 16 + 24.5, 8192 x 6001 45 + 113 -> 45 + 72, 4096 x 16383 71 + 148 -> 60 + 109.
   template <typename T> struct Raw {
     static constexpr int PIECES = (int)sizeof(T) / 2, PER = 16 / (int)sizeof(T);  // 16-byte pieces a chunk, elements a piece
     u32x4 p[NCH][PIECES];
@@ -106,6 +110,10 @@ struct Cols {
 #pragma unroll
           for (int k = 0; k < PIECES; ++k)
             p[i][k] = *reinterpret_cast<const typename Loose<T>::type*>(row + c + k * PER);
+        } else if (H >= 8) {
+#pragma unroll
+          for (int k = 0; k < PIECES; ++k)
+            p[i][k] = *reinterpret_cast<const typename Loose<T>::type*>(row + H - 8 + k * PER);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -118,14 +126,23 @@ struct Cols {
         }
       }
     }
-    __device__ __forceinline__ void unpack(float (&v)[NCH][8]) const {
+    __device__ __forceinline__ void unpack(int t, int H, float (&v)[NCH][8]) const {
 #pragma unroll
-      for (int i = 0; i < NCH; ++i)
+      for (int i = 0; i < NCH; ++i) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if constexpr (sizeof(T) == 4) v[i][e] = __uint_as_float(p[i][e / 4][e % 4]);
           else v[i][e] = e % 2 ? Fmt16<T>::hi(p[i][0][e / 2]) : Fmt16<T>::lo(p[i][0][e / 2]);
         }
+        const int c = at(t, i), down = c + 8 - H;
+        if (!VEC && H >= 8 && c < H && down > 0) {
+#pragma unroll
+          for (int by = 4; by > 0; by /= 2)
+            if (down & by)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[i][e] = e + by < 8 ? v[i][e + by] : 0.0f;
+        }
+      }
     }
   };
 };
@@ -179,7 +196,7 @@ __global__ __launch_bounds__(kLnBlock) void layernorm_fwd_kernel(const TX* __res
   for (int64_t base = (int64_t)blockIdx.x * RPB, row = first; base < T_; base += step, row += step) {  // uniform over the block
     float v[NCH][8];
     if (!AHEAD && row < T_) next.load(x + row * H, t, H);
-    next.unpack(v);
+    next.unpack(t, H, v);
     if (AHEAD && row + step < T_) next.load(x + (row + step) * H, t, H);
     float a[1] = {0.0f};
 #pragma unroll
@@ -221,7 +238,7 @@ __global__ __launch_bounds__(kLnBlock) void layernorm_fwd_kernel(const TX* __res
 // blocks of eight waves a compute unit, no more. 8192 x 2048 bf16: 21.5 us, 101 MB
 // at 4.7 TB/s; 16384 x 4096: 84 us, 403 MB at 4.8; 1531 x 1001 fp32: 9.6 us.
 template <typename TX, typename TG, int WPR, int NCH, bool VEC>
-__global__ __launch_bounds__(kLnBlock) void layernorm_bwd_kernel(const TG* __restrict__ g, const TX* __restrict__ x,
+__global__ __launch_bounds__(kLnBlock, sizeof(TX) == 2 && WPR <= 2 && NCH <= 2 ? 4 : 2) void layernorm_bwd_kernel(const TG* __restrict__ g, const TX* __restrict__ x,
                                                                  const void* __restrict__ w, int w_code,
                                                                  const float* __restrict__ mean,
                                                                  const float* __restrict__ rstd, int64_t T_, int H,
@@ -254,8 +271,8 @@ __global__ __launch_bounds__(kLnBlock) void layernorm_bwd_kernel(const TG* __res
   for (int64_t base = (int64_t)blockIdx.x * RPB, row = first; base < T_; base += step, row += step, ++turn) {  // uniform
     const bool on = row < T_;
     float xv[NCH][8], gv[NCH][8];
-    nx.unpack(xv);
-    ng.unpack(gv);
+    nx.unpack(t, H, xv);
+    ng.unpack(t, H, gv);
     const float mu = nmu, r = nr;
     if (row + step < T_) fetch(row + step);
     float s[2] = {0.0f, 0.0f};
@@ -435,33 +452,36 @@ hipError_t by_width_fwd(int H, bool vec, F&& f) {
   if (H <= 8192) return go(integral_constant<int, 8>(), integral_constant<int, 2>());
   return go(integral_constant<int, 8>(), integral_constant<int, 4>());
 }
-// The backward holds six values a column, in two chunks a thread up to 2048 columns
-// and beyond them for `narrow` rows (fp32, or a last chunk that may be cut), where
-// four would spill: 8192 x 2048 fp32, two / four chunks 38 / 42 us, fp32 with bf16
-// gradients 33 / 37; 4096 x 8192 bf16 46 / 45.
+// The backward holds six values a column, in two chunks a thread up to 2048 columns,
+// and beyond them where four would spill or gain nothing: fp32, 8192 x 2048, two /
+// four chunks 38 / 42 us, with bf16 gradients 33 / 37; rows of 16 bits that do not
+// start on 16 bytes up to 4096 columns, 8192 x 4001 39 / 43, but 8192 x 6001 80 / 72
+// (aligned: 16384 x 4096 82 / 80, 4096 x 8192 46 / 45).
 // 16-bit rows in two chunks leave room for two blocks a compute unit. Two / one (of
 // four chunks from 1025 columns on), with the sums' launch, bf16: 32768 x 512 24.0 /
-// 26.9 us, 32768 x 1024 40.4 / 42.1, 2048 x 2048 14.0 / 16.2, 8192 x 2048 25.4 / 27.5,
-// 8192 x 2001 26.0 / 31.1; but 16384 x 4096 82 / 80, 4096 x 8192 53 / 44, and fp32,
-// whose registers do not fit, 8192 x 2048 42 / 39.
-template <class F>
-hipError_t by_width_bwd(int H, bool vec, bool narrow, F&& f) {
+// 26.9 us, 32768 x 1024 40.4 / 42.1, 2048 x 2048 14.0 / 16.2, 8192 x 2048 25.4 / 27.5;
+// but 16384 x 4096 82 / 80, 4096 x 8192 53 / 44, and fp32, whose registers do not
+// fit, 8192 x 2048 42 / 39.
+template <bool HALF, class F>
+hipError_t by_width_bwd(int H, bool vec, F&& f) {
   using std::integral_constant;
   auto go = [&](auto wpr, auto nch) { return vec ? f(wpr, nch, std::true_type()) : f(wpr, nch, std::false_type()); };
   if (H <= 512) return go(integral_constant<int, 1>(), integral_constant<int, 1>());
   if (H <= 1024) return go(integral_constant<int, 1>(), integral_constant<int, 2>());
   if (H <= 2048) return go(integral_constant<int, 2>(), integral_constant<int, 2>());
-  if (narrow) {
+  if constexpr (HALF) {
+    if (H <= 4096)
+      return vec ? f(integral_constant<int, 2>(), integral_constant<int, 4>(), std::true_type())
+                 : f(integral_constant<int, 4>(), integral_constant<int, 2>(), std::false_type());
+    if (H <= 8192) return go(integral_constant<int, 4>(), integral_constant<int, 4>());
+  } else {
     if (H <= 4096) return go(integral_constant<int, 4>(), integral_constant<int, 2>());
     if (H <= 8192) return go(integral_constant<int, 8>(), integral_constant<int, 2>());
-  } else {
-    if (H <= 4096) return f(integral_constant<int, 2>(), integral_constant<int, 4>(), std::true_type());
-    if (H <= 8192) return f(integral_constant<int, 4>(), integral_constant<int, 4>(), std::true_type());
   }
   return go(integral_constant<int, 8>(), integral_constant<int, 4>());
 }
 
-// Rows that a block of the backward has at a time (narrow: as many, or half).
+// Rows that a block of the backward has at a time (in two chunks a thread: as many, or half).
 int rows_a_block(int H) { return H <= 2048 ? 8 : H <= 4096 ? 4 : H <= 8192 ? 2 : 1; }
 int64_t wide_rows(int64_t T_) { return std::max<int64_t>(kLnColRows, (T_ + kLnColBlocks - 1) / kLnColBlocks); }
 
@@ -515,7 +535,7 @@ hipError_t layernorm_bwd(const TG* g, const TX* x, const void* w, int w_code, co
                          s, g, x, mean, rstd, T_, H, wide_rows(T_), part, ld);
     st = hipGetLastError();
   } else if (T_ > 0) {
-    st = by_width_bwd(H, vec, !vec || sizeof(TX) == 4, [&](auto wpr, auto nch, auto v) {
+    st = by_width_bwd<sizeof(TX) == 2>(H, vec, [&](auto wpr, auto nch, auto v) {
       constexpr int WPR = decltype(wpr)::value, NCH = decltype(nch)::value;
       hipLaunchKernelGGL((layernorm_bwd_kernel<TX, TG, WPR, NCH, decltype(v)::value>), dim3(nb), dim3(kLnBlock), 0, s, g,
                          x, w, w_code, mean, rstd, T_, H, gx, part, ld);
